@@ -437,6 +437,90 @@ int dtt_clip_adamw_ex(const DttOptTensor* tab, int ntensors, const int32_t* chun
                       float max_norm, float beta1, float beta2, float eps, int step, const int32_t* step_dev,
                       const float* sumsq_dev, float grad_scale, float* norm_out, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Token mixers for long recordings (no counterpart in the reference, whose
+ * BiLSTM, dense token attention and additive sinusoids -- latent.py:87-96,
+ * cross_attention_positional.py:6-12,66-69 -- need the whole clip at once).
+ * dtype: 0 = float32, 1 = bfloat16, for every tensor without another type.
+ * Strides are in elements; the innermost axis is contiguous.
+ * ------------------------------------------------------------------------- */
+
+/* Gated linear recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a = sigmoid(f), y_t = h_t, over N = outer * NI items of L steps
+ * and D channels; item n reads x at (n / NI) * x_so + (n % NI) * x_si + step * x_sl (f, dy alike); y, dx, df are
+ * contiguous [N][L][D].  reverse: from an item's last step to its first.  lengths [N] (NULL: all L): steps from
+ * lengths[n] on are padding: never read, y = dx = df = 0 there, the state passes them.  h0 [N][D] (NULL: zero) starts
+ * every item; last [N][D] (may be NULL) receives the state behind its last step.  states: dtt_recurrence_states() floats,
+ * written by the forward call where not NULL and read by the backward call (same N, L, D, dtype and contents of x,
+ * f, h0, lengths, reverse).  Backward: dy and dlast [N][D] (NULL: zero) in; dx, df and dh0 [N][D] (may be NULL) out.
+ * ws: dtt_recurrence_ws_bytes() bytes for this call's pointers and strides (0: none needed), undefined afterwards. */
+typedef struct {
+    const void* x; const void* f; const void* dy;
+    void* y; void* dx; void* df;
+    const float* h0; const float* dlast; float* last; float* dh0;
+    float* states; const int32_t* lengths;
+    void* ws; int64_t ws_bytes;
+    int64_t x_so, x_si, x_sl, f_so, f_si, f_sl, g_so, g_si, g_sl;
+    int32_t N, NI, L, D, reverse, dtype;
+} DttRecurrence;
+int64_t dtt_recurrence_ws_bytes(const DttRecurrence* g);
+int64_t dtt_recurrence_states(const DttRecurrence* g);
+int dtt_recurrence_fwd(const DttRecurrence* g, void* stream);
+int dtt_recurrence_bwd(const DttRecurrence* g, void* stream);
+/* One step: state [N][D] fp32 (contiguous) is replaced, y [N][D] (contiguous) is the new state in dtype; x, f rows x_sn,
+ * f_sn apart. */
+int dtt_recurrence_step(const void* x, const void* f, float* state, void* y, int N, int D, int64_t x_sn, int64_t f_sn, int dtype,
+                        void* stream);
+
+/* Rotary positions: in every head of q [B][T][Hq][dh] and k [B][T][Hk][dh] (Hk = 0: q alone) the pairs of the first r
+ * channels -- (i, i + r/2), or (2i, 2i + 1) when interleaved -- are turned by position * freq[i] and scaled by
+ * amplitude; the other channels are copied.  back: turned the other way (the gradient).  positions: int32 or (pos64) int64
+ * at b * p_sb + t * p_st; freq: r/2 doubles, radians per position.  qo, ko: contiguous. */
+typedef struct {
+    const void* q; const void* k; void* qo; void* ko;
+    const void* positions; const double* freq;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, p_sb, p_st;
+    int32_t B, T, Hq, Hk, dh, r, interleaved, back, pos64, dtype;
+    float amplitude;
+    int32_t reserved_;
+} DttRotary;
+int dtt_rotary(const DttRotary* g, void* stream);
+
+/* Windowed attention with first tokens that stay visible: the query at position p = offset + i sees key j where
+ * j <= p + right and (j >= p - left or j < sinks); softmax(scale * q k^T) v over those; a row that sees none is zero.
+ * lengths [B] (NULL: none): positions from lengths[b] on are padding: keys there are never read, rows there are zero and
+ * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides, every row on 16 bytes; out, dq
+ * [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
+ * lse [B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call; dd: the same size, scratch of
+ * the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give equal bits. */
+typedef struct {
+    const void* q; const void* k; const void* v; void* out; float* lse;
+    const void* dout; void* dq; void* dk; void* dv; float* dd;
+    const int32_t* lengths; void* ws; int64_t ws_bytes;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
+    int32_t B, Tq, Tk, Hq, Hk, DH, left, right, sinks, offset, dtype;
+    float scale;
+} DttWattn;
+int dtt_wattn_fwd(const DttWattn* g, void* stream);
+int64_t dtt_wattn_bwd_ws_bytes(const DttWattn* g);
+int dtt_wattn_bwd(const DttWattn* g, void* stream);
+
+/* One token per item against a rolling cache kc, vc [B][S + W][Hk][DH] (by strides) that holds the first S positions and the
+ * last W: position p lives in slot p < S ? p : S + (p - S) % W.  The step writes k, v [B][Hk][DH] of position positions[b]
+ * (int64, device memory) into its slot and attends q [B][Hq][DH] to every slot filled so far, out [B][Hq][DH] contiguous.
+ * An item with a negative position is idle: its cache stays as it is and its row is zero.  ws: dtt_wattn_step_ws_bytes().
+ * dtt_wattn_cache_fill: what the cache of item b holds after the first lengths[b] (NULL: Tn) positions of k, v
+ * [B][Tn][Hk][DH]; slots that hold none of them stay as they are (q, out, positions, ws unused). */
+typedef struct {
+    const void* q; const void* k; const void* v; void* kc; void* vc; void* out;
+    const int64_t* positions; void* ws; int64_t ws_bytes;
+    int64_t q_sb, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+    int32_t B, Hq, Hk, DH, S, W, dtype;
+    float scale;
+} DttWattnStep;
+int64_t dtt_wattn_step_ws_bytes(const DttWattnStep* g);
+int dtt_wattn_step(const DttWattnStep* g, void* stream);
+int dtt_wattn_cache_fill(const DttWattnStep* g, const int32_t* lengths, int Tn, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

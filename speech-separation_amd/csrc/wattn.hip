@@ -1,0 +1,849 @@
+// Windowed attention with first tokens that stay visible.  The query at position p = offset + i sees the key at position j
+// where  j <= p + right  and  (j >= p - left  or  j < sinks)  and  j < len;  positions from len on are padding (rows of
+// zeros, no gradient); a row that sees nothing is a row of zeros.  q [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides, Hq a
+// multiple of Hk (query head h reads key head h / (Hq / Hk)), bf16 or fp32.
+//
+// One pass over the visible key tiles with the running maximum and sum of the softmax in fp32 (base 2: one v_exp_f32 a
+// score).  Scores are formed transposed, S^T = K Q^T on 32x32 matrix tiles: a lane then owns one query (column lane & 31),
+// so that the softmax statistics are per-lane scalars and one exchange with lane ^ 32, and the tile's accumulator
+// registers, packed to the compute type, already are the B operand of O^T += V^T P^T: register r of a 16-key chunk holds key
+// (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and V^T's fragments are read from LDS in that order of keys.
+// P and dS are rounded to the compute type there (bf16: half a step 2^-9 relative each, at the size of the outputs' own
+// rounding); statistics, accumulators, D = sum(dO O) and sinks' partial sums stay fp32.
+//
+// Bound: the matrix cores (4 DH flops per visible pair forward, 10 DH backward) for windows beyond a few hundred keys, HBM
+// below.
+#include "common.h"
+#include "../../include/dtt_hip.h"
+
+namespace {
+constexpr int NTH = 256, BM = 128, BN = 64;      // forward / dq: query rows of a workgroup (32 a wave), keys of a staged tile
+constexpr int KM = 128, QN = 64;                 // dk / dv: keys of a workgroup (32 a wave), query rows of a staged tile
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct WaP {
+    const void* q; const void* k; const void* v; const void* o; const void* dout;
+    void* out; void* dq; void* dk; void* dv;
+    float* lse; float* dd; float* part;
+    const int* len;
+    int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
+    int B, Tq, Tk, Hq, Hk, G, left, right, sinks, offset;
+    int nt, nchunk, chunk, npart;                // tiles along the row axis; far-query chunks of the sinks' gradients
+    float scale;
+};
+
+// LDS image of rows of DH elements in 16-byte pieces; piece c of row r is stored at c ^ swz(r).  Rows are a power of two of
+// pieces.  swz spreads both reads over all 64 banks: the natural fragment read (16 rows, one piece each) and the
+// transposing read (four consecutive rows, four neighbouring pieces).
+template <typename T, int DH> struct Img {
+    static constexpr int EPP = 16 / sizeof(T), NP = DH / EPP;
+    static constexpr int RP = NP <= 4 ? 4 : NP <= 8 ? 8 : NP <= 16 ? 16 : NP <= 32 ? 32 : 64, LD = RP * EPP;
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (RP >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+        else if constexpr (RP == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else return (r >> 2) & 3;
+    }
+    static __device__ __forceinline__ int at(int r, int piece) { return r * LD + (piece ^ swz(r)) * EPP; }
+};
+
+// natural fragment: row r, the 8 elements from 16 c + 8 lh on
+template <typename T, int DH> __device__ __forceinline__ typename MM<T>::Frag nat_frag(const T* img, int r, int c, int lh) {
+    if constexpr (sizeof(T) == 2) {
+        return MM<T>::ldfrag(img + Img<T, DH>::at(r, 2 * c + lh));
+    } else {
+        typename MM<T>::Frag f;
+        f.lo = *reinterpret_cast<const float4*>(img + Img<T, DH>::at(r, 4 * c + 2 * lh));
+        f.hi = *reinterpret_cast<const float4*>(img + Img<T, DH>::at(r, 4 * c + 2 * lh + 1));
+        return f;
+    }
+}
+// transposed fragment: column c0 + (lane & 31), rows kb + (e & 3) + 8 (e >> 2) + 4 lh for e = 0 .. 7
+template <typename T, int DH> __device__ __forceinline__ typename MM<T>::Frag tr_frag_of(const T* img, int kb, int c0) {
+    const int lane = threadIdx.x & 63, lh = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        const int g = (lane >> 4) & 1, q = (lane & 15) >> 2, p = lane & 3, piece = c0 / 8 + 2 * g + (p >> 1), r = kb + 4 * lh + q;
+        return tr_frag(img + Img<T, DH>::at(r, piece) + 4 * (p & 1), img + Img<T, DH>::at(r + 8, piece) + 4 * (p & 1));
+    } else {
+        const int d = c0 + (lane & 31);
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = img[Img<T, DH>::at(kb + (i & 3) + 8 * (i >> 2) + 4 * lh, d >> 2) + (d & 3)];
+        typename MM<T>::Frag f;
+        f.lo = make_float4(e[0], e[1], e[2], e[3]);
+        f.hi = make_float4(e[4], e[5], e[6], e[7]);
+        return f;
+    }
+}
+// accumulator registers 8 c .. 8 c + 7 as an operand fragment
+template <typename T> __device__ __forceinline__ typename MM<T>::Frag acc_frag(const f32x16_t& s, int c) {
+    if constexpr (sizeof(T) == 2) {
+        uint4 u = make_uint4(pack_bf16x2(s[8 * c], s[8 * c + 1]), pack_bf16x2(s[8 * c + 2], s[8 * c + 3]),
+                             pack_bf16x2(s[8 * c + 4], s[8 * c + 5]), pack_bf16x2(s[8 * c + 6], s[8 * c + 7]));
+        return __builtin_bit_cast(s16x8_t, u);
+    } else {
+        typename MM<T>::Frag f;
+        f.lo = make_float4(s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3]);
+        f.hi = make_float4(s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]);
+        return f;
+    }
+}
+__device__ __forceinline__ f32x16_t zero_acc() {
+    f32x16_t z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+__device__ __forceinline__ int acc_row(int r, int lh) { return (r & 3) + 8 * (r >> 2) + 4 * lh; }
+
+// R rows from `src` (row stride rs elements) into registers; rows outside [0, n) come from the zero page, never from memory
+template <typename T, int DH, int R> struct Stage {
+    static constexpr int NP = Img<T, DH>::NP, N = (R * NP + NTH - 1) / NTH;
+    Vec16<T> v[N];
+    __device__ __forceinline__ void load(const T* src, int64_t rs, int r0, int n) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = threadIdx.x + i * NTH, r = r0 + id / NP;
+            v[i] = ld16_pred<T>(src + (int64_t)r * rs + (id % NP) * Img<T, DH>::EPP, src, id < R * NP && r >= 0 && r < n);
+        }
+    }
+    __device__ __forceinline__ void store(T* img) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int id = threadIdx.x + i * NTH;
+            if (R * NP % NTH == 0 || id < R * NP) st16<T>(img + Img<T, DH>::at(id / NP, id % NP), v[i]);
+        }
+    }
+};
+
+// consecutive logical workgroups on one XCD (workgroup id % 8): the heads of a group and neighbouring tiles share keys
+__device__ __forceinline__ int xcd_order(int id, int n) {
+    const int per = n / 8;
+    return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
+// 4 consecutive channels per register group of an O^T-shaped accumulator: row pointer + 32 ct + 8 q + 4 lh
+template <typename T, int DH>
+__device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32], float mul, int lh) {
+#pragma unroll
+    for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            T* o = row + 32 * ct + 8 * q + 4 * lh;
+            const float a = acc[ct][4 * q] * mul, b = acc[ct][4 * q + 1] * mul, c = acc[ct][4 * q + 2] * mul, d = acc[ct][4 * q + 3] * mul;
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+            else *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+        }
+}
+
+// The key tiles (of N keys) that the query rows at positions p0 .. p1 see: [0, a) holds first tokens only, [b, c] the window.
+struct Tiles { int a, b, c; };
+template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0, int p1, int klen) {
+    Tiles t{0, 0, -1};
+    if (p1 < p0 || klen <= 0) return t;
+    const int jmax = min(p1 + p.right, klen - 1), jmin = max(0, p0 - p.left), ns = min(p.sinks, jmax + 1);
+    if (jmax < 0) return t;
+    t.a = (ns + N - 1) / N;
+    if (jmin <= jmax) t.b = jmin / N, t.c = jmax / N, t.a = min(t.a, t.b);
+    else t.b = t.a, t.c = t.a - 1;
+    return t;
+}
+
+template <typename T, int DH>
+__global__ __launch_bounds__(NTH) void wattn_fwd_kernel(const WaP p) {
+    typedef Img<T, DH> I;
+    typedef typename MM<T>::Frag Frag;
+    __shared__ __align__(16) T ks[BN * I::LD];
+    __shared__ __align__(16) T vs[BN * I::LD];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int g = id % p.G; id /= p.G;
+    const int qt = id % p.nt; id /= p.nt;
+    const int hk = id % p.Hk, b = id / p.Hk, h = hk * p.G + g;
+    const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
+    const int i = qt * BM + wave * 32 + lr, pos = p.offset + i, pw = p.offset + qt * BM + wave * 32;
+    const T* q = (const T*)p.q + b * p.q_sb + (int64_t)min(i, p.Tq - 1) * p.q_st + h * p.q_sh;
+    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    Frag qf[DH / 16];
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
+    f32x16_t o[DH / 32];
+#pragma unroll
+    for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
+    float m = -INFINITY, l = 0.f;
+    const float sc = p.scale * LOG2E;
+
+    const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
+    const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
+    Stage<T, DH, BN> sk, sv;
+    int t = tl.a > 0 ? 0 : tl.b;
+    const int count = tl.a + tl.c - tl.b + 1;
+    if (count > 0) {
+        sk.load(k, p.k_st, t * BN, klen);
+        sv.load(v, p.v_st, t * BN, klen);
+    }
+    for (int n = 0; n < count; ++n) {
+        __syncthreads();
+        sk.store(ks);
+        sv.store(vs);
+        __syncthreads();
+        const int j0 = t * BN;
+        t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
+        if (n + 1 < count) {
+            sk.load(k, p.k_st, t * BN, klen);
+            sv.load(v, p.v_st, t * BN, klen);
+        }
+#pragma unroll
+        for (int s = 0; s < BN / 32; ++s) {
+            const int js = j0 + 32 * s;
+            // nothing of this 32 x 32 tile is visible
+            if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
+            f32x16_t x = zero_acc();
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
+            const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
+            if (!full) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = js + acc_row(r, lh);
+                    const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
+                    x[r] = see ? x[r] : -INFINITY;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+            const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
+            const float al = __builtin_amdgcn_exp2f(m - mu);
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
+                sum += x[r];
+            }
+            l = fmaf(l, al, sum);
+            m = mn;
+            if (__any(al != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < DH / 32; ++c)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[c][r] *= al;
+            }
+            const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+#pragma unroll
+            for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(vs, 32 * s + 16 * c, 32 * ct), pf[c], o[ct]);
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (i >= p.Tq) return;
+    const bool live = pos < qlen && l != 0.f;         // (l is at least 1 where anything is visible; NaN passes)
+    T* out = (T*)p.out + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH;
+    if (!live) {
+#pragma unroll
+        for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
+    }
+    store_rows<T, DH>(out, o, live ? 1.f / l : 0.f, lh);
+    if (p.lse && lh == 0) p.lse[((int64_t)b * p.Hq + h) * p.Tq + i] = live ? m + log2f(l) : INFINITY;
+}
+
+// dq, and D = sum(dO O) per row for the dk / dv launch behind it
+template <typename T, int DH>
+__global__ __launch_bounds__(NTH) void wattn_dq_kernel(const WaP p) {
+    typedef Img<T, DH> I;
+    typedef typename MM<T>::Frag Frag;
+    __shared__ __align__(16) T ks[BN * I::LD];
+    __shared__ __align__(16) T vs[BN * I::LD];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int g = id % p.G; id /= p.G;
+    const int qt = id % p.nt; id /= p.nt;
+    const int hk = id % p.Hk, b = id / p.Hk, h = hk * p.G + g;
+    const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
+    const int i = qt * BM + wave * 32 + lr, ic = min(i, p.Tq - 1), pos = p.offset + i, pw = p.offset + qt * BM + wave * 32;
+    const bool live = i < p.Tq && pos < qlen;
+    const T* q = (const T*)p.q + b * p.q_sb + (int64_t)ic * p.q_st + h * p.q_sh;
+    const T* go = (const T*)p.dout + b * p.g_sb + (int64_t)ic * p.g_st + h * p.g_sh;
+    const T* oo = (const T*)p.o + ((int64_t)(b * p.Tq + ic) * p.Hq + h) * DH;
+    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    Frag qf[DH / 16], gf[DH / 16];
+    float dd = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) {
+        qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
+        gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
+        const T* a = reinterpret_cast<const T*>(&gf[c]);
+        const Frag of = MM<T>::ldfrag(oo + 16 * c + 8 * lh);
+        const T* z = reinterpret_cast<const T*>(&of);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dd = fmaf(ldf(a + e), ldf(z + e), dd);
+    }
+    dd += __shfl_xor(dd, 32, 64);
+    const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
+    const float lse = p.lse[at];
+    if (live && lh == 0) p.dd[at] = dd;
+    f32x16_t dq[DH / 32];
+#pragma unroll
+    for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
+    const float sc = p.scale * LOG2E;
+    const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
+    const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
+    Stage<T, DH, BN> sk, sv;
+    int t = tl.a > 0 ? 0 : tl.b;
+    const int count = tl.a + tl.c - tl.b + 1;
+    if (count > 0) {
+        sk.load(k, p.k_st, t * BN, klen);
+        sv.load(v, p.v_st, t * BN, klen);
+    }
+    for (int n = 0; n < count; ++n) {
+        __syncthreads();
+        sk.store(ks);
+        sv.store(vs);
+        __syncthreads();
+        const int j0 = t * BN;
+        t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
+        if (n + 1 < count) {
+            sk.load(k, p.k_st, t * BN, klen);
+            sv.load(v, p.v_st, t * BN, klen);
+        }
+#pragma unroll
+        for (int s = 0; s < BN / 32; ++s) {
+            const int js = j0 + 32 * s;
+            if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
+            f32x16_t x = zero_acc(), y = zero_acc();
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
+            const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = js + acc_row(r, lh);
+                const bool see = full || (j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen);
+                const float e = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse));
+                x[r] = see ? e * (y[r] - dd) : 0.f;
+            }
+            const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+#pragma unroll
+            for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct), pf[c], dq[ct]);
+        }
+    }
+    if (i >= p.Tq) return;
+    if (!live || lse == INFINITY) {
+#pragma unroll
+        for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
+    }
+    store_rows<T, DH>((T*)p.dq + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH, dq, p.scale, lh);
+}
+
+// dk, dv: a workgroup owns KM keys of one key head (32 a wave) and walks the query rows that see them, over the heads of its
+// group: no atomics, one order of additions.  First tokens are seen by every later row: the rows beyond the window of
+// tile 0 are cut into chunks, each a workgroup of its own (blockIdx.x >= main) whose waves 0 and 1 take every other
+// 32-row tile against the first tokens' rows; those and tile 0's own sums go to fp32 partials that
+// wattn_sink_sum_kernel adds in order.
+template <typename T, int DH>
+__global__ __launch_bounds__(NTH) void wattn_dkv_kernel(const WaP p, int main) {
+    typedef Img<T, DH> I;
+    typedef typename MM<T>::Frag Frag;
+    __shared__ __align__(16) T qs[QN * I::LD];
+    __shared__ __align__(16) T gs[QN * I::LD];
+    __shared__ __align__(16) float st[2][QN];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    const bool far = (int)blockIdx.x >= main;
+    int id = far ? blockIdx.x - main : xcd_order(blockIdx.x, main);
+    const int ns32 = (p.sinks + 31) / 32;
+    int kt = 0, ch = 0, kw;                       // key tile; chunk; first key of this wave
+    if (far) {
+        ch = id % p.nchunk; id /= p.nchunk;
+        kw = id % ns32 * 32; id /= ns32;
+    } else {
+        kt = id % p.nt; id /= p.nt;
+        kw = kt * KM + wave * 32;
+    }
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
+    const int qrows = min(p.Tq, qlen < INT_MAX ? max(0, qlen - p.offset) : p.Tq);       // live query rows
+    // query rows of this workgroup: [r0, r1)
+    const int edge = min(p.Tq, max(0, KM + p.left - p.offset));          // first row beyond the window of tile 0
+    int r0, r1;
+    if (far) {
+        r0 = edge + ch * p.chunk;
+        r1 = min(r0 + p.chunk, qrows);
+    } else {
+        r0 = max(0, kt * KM - p.right - p.offset);
+        r1 = min(qrows, max(0, kt * KM + KM + p.left - p.offset));
+    }
+    const int j = kw + lr, jc = min(j, p.Tk - 1);
+    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh + (int64_t)jc * p.k_st;
+    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh + (int64_t)jc * p.v_st;
+    Frag kf[DH / 16], vf[DH / 16];
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) {
+        kf[c] = MM<T>::ldfrag(k + 16 * c + 8 * lh);
+        vf[c] = MM<T>::ldfrag(v + 16 * c + 8 * lh);
+    }
+    f32x16_t dk[DH / 32], dv[DH / 32];
+#pragma unroll
+    for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
+    const float sc = p.scale * LOG2E;
+    Stage<T, DH, QN> sq, sg;
+    const int per = r1 > r0 ? (r1 - r0 + QN - 1) / QN : 0, count = per * p.G;
+    float sl = 0.f, sd = 0.f;
+    auto load = [&](int n) {
+        const int h = hk * p.G + n / per, r = r0 + n % per * QN;
+        sq.load((const T*)p.q + b * p.q_sb + h * p.q_sh, p.q_st, r, r1);
+        sg.load((const T*)p.dout + b * p.g_sb + h * p.g_sh, p.g_st, r, r1);
+        if (threadIdx.x < QN) {
+            const int i = r + threadIdx.x;
+            const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + min(i, p.Tq - 1);
+            const float lv = p.lse[at], dvv = p.dd[at];
+            sl = i < r1 ? lv : INFINITY;
+            sd = i < r1 ? dvv : 0.f;
+        }
+    };
+    if (count > 0) load(0);
+    for (int n = 0; n < count; ++n) {
+        __syncthreads();
+        sq.store(qs);
+        sg.store(gs);
+        if (threadIdx.x < QN) st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd;
+        __syncthreads();
+        const int i0 = r0 + n % per * QN;
+        if (n + 1 < count) load(n + 1);
+#pragma unroll
+        for (int s = 0; s < QN / 32; ++s) {
+            if (far && s != wave) continue;
+            const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
+            if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
+            f32x16_t x = zero_acc(), y = zero_acc();
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), kf[c], x);
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
+            const bool full = kw + 31 <= pr + p.right && (kw >= pr + 31 - p.left || kw + 31 < p.sinks) && kw + 31 < klen;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const float4 ls = *reinterpret_cast<const float4*>(&st[0][32 * s + 8 * r4 + 4 * lh]);
+                const float4 ds = *reinterpret_cast<const float4*>(&st[1][32 * s + 8 * r4 + 4 * lh]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * r4 + e, pp = pr + 8 * r4 + 4 * lh + e;
+                    const bool see = full || (j <= pp + p.right && (j >= pp - p.left || j < p.sinks) && j < klen);
+                    const float pv = see ? __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(&ls.x)[e])) : 0.f;
+                    x[r] = pv;
+                    y[r] = see ? pv * (y[r] - (&ds.x)[e]) : 0.f;
+                }
+            }
+            const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+            const Frag df[2] = {acc_frag<T>(y, 0), acc_frag<T>(y, 1)};
+#pragma unroll
+            for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    MM<T>::mma(tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct), pf[c], dv[ct]);
+                    MM<T>::mma(tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct), df[c], dk[ct]);
+                }
+        }
+    }
+    if (p.nchunk > 0 && j < p.sinks && (!far || wave < 2)) {              // first tokens: fp32 partials, summed in order behind
+        const int at = far ? 1 + 2 * ch + wave : 0;
+        float* d = p.part + ((((int64_t)b * p.Hk + hk) * p.npart + at) * p.sinks + j) * 2 * DH;
+        store_rows<float, DH>(d, dk, p.scale, lh);
+        store_rows<float, DH>(d + DH, dv, 1.f, lh);
+    }
+    if (far || j >= p.Tk || (p.nchunk > 0 && j < p.sinks)) return;
+    const int64_t row = ((int64_t)(b * p.Tk + j) * p.Hk + hk) * DH;
+    store_rows<T, DH>((T*)p.dk + row, dk, p.scale, lh);
+    store_rows<T, DH>((T*)p.dv + row, dv, 1.f, lh);
+}
+
+// first tokens' dk, dv: the partials in their order
+template <typename T>
+__global__ __launch_bounds__(NTH) void wattn_sink_sum_kernel(const WaP p, int dh, int64_t n) {
+    const int64_t id = (int64_t)blockIdx.x * NTH + threadIdx.x;
+    if (id >= n) return;
+    const int d = (int)(id % (2 * dh));
+    const int64_t bj = id / (2 * dh);
+    const int j = (int)(bj % p.sinks);
+    const int64_t bh = bj / p.sinks;
+    const float* s = p.part + (bh * p.npart * p.sinks + j) * 2 * dh + d;
+    float sum = 0.f;
+    for (int k = 0; k < p.npart; ++k) sum += s[(int64_t)k * p.sinks * 2 * dh];
+    if (j >= p.Tk) return;
+    const int64_t row = ((bh / p.Hk * p.Tk + j) * p.Hk + bh % p.Hk) * dh;
+    if (d < dh) stf((T*)p.dk + row + d, sum);
+    else stf((T*)p.dv + row + d - dh, sum);
+}
+
+// ---- one token against a rolling cache -------------------------------------------------------------------------------
+struct WsP {
+    const void* q; const void* k; const void* v; void* kc; void* vc; void* out;
+    const int64_t* pos;
+    float* part;                                  // [B][Hk][ngrp][nsplit][32][DH + 2]: o (unnormalised), m, l
+    int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+    int B, Hq, Hk, G, ngrp, S, W, nsplit, per;    // per: slots of a split (a multiple of 128)
+    float scale;
+};
+
+__device__ __forceinline__ int slot_of(int64_t pos, int S, int W) { return pos < S ? (int)pos : S + (int)((pos - S) % W); }
+
+// A workgroup takes one item, one key head (all its query heads at once: the columns of the matrix tile) and one range of
+// slots; a wave takes every fourth 32-slot tile of it.  K is read from memory in fragment order; V goes through
+// a wave's own LDS image for the transposing read.
+template <typename T, int DH>
+__global__ __launch_bounds__(NTH) void wattn_step_kernel(const WsP p) {
+    typedef Img<T, DH> I;
+    typedef typename MM<T>::Frag Frag;
+    constexpr int NV = (32 * I::NP + 63) / 64;
+    __shared__ __align__(16) T vs[4][32 * I::LD];
+    __shared__ float ml[4][2][32];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    int id = blockIdx.x;
+    const int split = id % p.nsplit; id /= p.nsplit;
+    const int grp = id % p.ngrp; id /= p.ngrp;
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const int64_t pos = p.pos[b];
+    const int M = p.S + p.W;
+    const int valid = pos < 0 ? 0 : (int)min((int64_t)M, pos + 1), cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
+    const int hg = grp * 32 + lr, h = hk * p.G + min(hg, p.G - 1);
+    const T* q = (const T*)p.q + b * p.q_sb + h * p.q_sh;
+    const T* kn = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* vn = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    T* kc = (T*)p.kc + b * p.kc_sb + hk * p.kc_sh;
+    T* vc = (T*)p.vc + b * p.vc_sb + hk * p.vc_sh;
+    const int s0 = split * p.per, s1 = min(valid, s0 + p.per);
+    if (grp == 0 && cur >= s0 && cur < s0 + p.per && wave == 3 && lane < I::NP) {
+        // the new token's rows; every reader of this slot takes them from k, v instead
+        st16<T>(kc + (int64_t)cur * p.kc_st + lane * I::EPP, ld16<T>(kn + lane * I::EPP));
+        st16<T>(vc + (int64_t)cur * p.vc_st + lane * I::EPP, ld16<T>(vn + lane * I::EPP));
+    }
+    Frag qf[DH / 16];
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
+    f32x16_t o[DH / 32];
+#pragma unroll
+    for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
+    float m = -INFINITY, l = 0.f;
+    const float sc = p.scale * LOG2E;
+    Frag kf[DH / 16];
+    Vec16<T> vv[NV];
+    auto load = [&](int js) {
+        const int j = js + lr;
+        const T* kr = j == cur ? kn : kc + (int64_t)min(j, M - 1) * p.kc_st;
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) kf[c] = MM<T>::ldfrag(kr + 16 * c + 8 * lh);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 64 * i, r = e / I::NP, jj = js + r, pc = e % I::NP * I::EPP;
+            vv[i] = ld16_pred<T>(jj == cur ? vn + pc : vc + (int64_t)jj * p.vc_st + pc, vn, r < 32 && jj < valid);
+        }
+    };
+    int js = s0 + wave * 32;
+    if (js < s1) load(js);
+    for (; js < s1; js += 128) {
+        f32x16_t x = zero_acc();
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) MM<T>::mma(kf[c], qf[c], x);
+        T* img = vs[wave];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 64 * i;
+            if (32 * I::NP % 64 == 0 || e < 32 * I::NP) st16<T>(img + I::at(e / I::NP, e % I::NP), vv[i]);
+        }
+        if (js + 128 < s1) load(js + 128);
+        if (js + 31 >= valid) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = js + acc_row(r, lh) < valid ? x[r] : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+        const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
+        const float al = __builtin_amdgcn_exp2f(m - mu);
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
+            sum += x[r];
+        }
+        l = fmaf(l, al, sum);
+        m = mn;
+        if (__any(al != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < DH / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[c][r] *= al;
+        }
+        const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the image's writes ahead of its reads (one wave)
+#pragma unroll
+        for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(img, 16 * c, 32 * ct), pf[c], o[ct]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // and its reads ahead of the next writes
+    }
+    l += __shfl_xor(l, 32, 64);
+    // the four waves' states into one: weights 2^(m_w - m), channels of a column summed over the waves through LDS
+    if (lh == 0) ml[wave][0][lr] = m, ml[wave][1][lr] = l;
+    __syncthreads();
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ml[w][0][lr]);
+    const float mu = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) lt = fmaf(ml[w][1][lr], __builtin_amdgcn_exp2f(ml[w][0][lr] - mu), lt);
+    const float wt = __builtin_amdgcn_exp2f(m - mu);
+    float* acc = reinterpret_cast<float*>(&vs[0][0]);                    // [G' columns][DH], G' = min(32, heads of this block)
+    const int cols = min(32, p.G - grp * 32);
+    constexpr int FIT = (int)(sizeof(T) * 4 * 32 * I::LD / (4 * DH));    // columns that fit: at least 32 (4 images of 32 rows)
+    static_assert(FIT >= 32, "the image holds one fp32 row per column");
+    for (int w = 0; w < 4; ++w) {
+        __syncthreads();
+        if (wave == w && lr < cols) {
+#pragma unroll
+            for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float* d = acc + lr * DH + 32 * ct + acc_row(r, lh);
+                    const float add = o[ct][r] * wt;
+                    *d = w ? *d + add : add;
+                }
+        }
+    }
+    __syncthreads();
+    const int64_t bh = (int64_t)b * p.Hk + hk;
+    if (wave == 0 && lh == 0) ml[0][0][lr] = mt, ml[0][1][lr] = lt;
+    __syncthreads();
+    for (int e = threadIdx.x; e < cols * DH; e += NTH) {
+        const int c = e / DH, d = e % DH;
+        if (p.nsplit == 1) {
+            const float lv = ml[0][1][c];
+            stf((T*)p.out + ((int64_t)b * p.Hq + hk * p.G + grp * 32 + c) * DH + d, lv != 0.f ? acc[e] / lv : 0.f);
+        } else {
+            float* w = p.part + (((bh * p.ngrp + grp) * p.nsplit + split) * 32 + c) * (DH + 2);
+            w[d] = acc[e];
+            if (d < 2) w[DH + d] = ml[0][d][c];
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NTH) void wattn_step_join_kernel(const WsP p, int dh) {
+    const int64_t id = (int64_t)blockIdx.x * NTH + threadIdx.x;
+    if (id >= (int64_t)p.B * p.Hq * dh) return;
+    const int d = (int)(id % dh), h = (int)(id / dh % p.Hq);
+    const int64_t b = id / dh / p.Hq;
+    const int hk = h / p.G, g = h % p.G;
+    const float* w = p.part + (((b * p.Hk + hk) * p.ngrp + g / 32) * p.nsplit * 32 + g % 32) * (dh + 2);
+    const int64_t ss = 32ll * (dh + 2);
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, w[s * ss + dh]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float e = __builtin_amdgcn_exp2f(w[s * ss + dh] - mu);
+        l = fmaf(w[s * ss + dh + 1], e, l);
+        o = fmaf(w[s * ss + d], e, o);
+    }
+    stf((T*)p.out + id, l != 0.f ? o / l : 0.f);
+}
+
+// rows of a whole sequence that its cache holds after position len - 1: the first S and the last W
+template <typename T>
+__global__ __launch_bounds__(NTH) void wattn_fill_kernel(const WsP p, const int* len, int Tn, int64_t k_st, int64_t v_st, int np, int64_t n) {
+    constexpr int EPP = 16 / sizeof(T);
+    const int64_t id = (int64_t)blockIdx.x * NTH + threadIdx.x;
+    if (id >= n) return;
+    const int pc = (int)(id % np) * EPP, M = p.S + p.W;
+    int64_t r = id / np;
+    const int hk = (int)(r % p.Hk);
+    r /= p.Hk;
+    const int slot = (int)(r % M), b = (int)(r / M), L = len ? min(max(len[b], 0), Tn) : Tn;
+    int64_t t = slot;                             // the last position that lives in this slot
+    if (slot >= p.S && L > slot) t = slot + (int64_t)(L - 1 - slot) / p.W * p.W;
+    if (t >= L) return;                           // never written: left as it was
+    st16<T>((T*)p.kc + b * p.kc_sb + slot * p.kc_st + hk * p.kc_sh + pc, ld16<T>((const T*)p.k + b * p.k_sb + t * k_st + hk * p.k_sh + pc));
+    st16<T>((T*)p.vc + b * p.vc_sb + slot * p.vc_st + hk * p.vc_sh + pc, ld16<T>((const T*)p.v + b * p.v_sb + t * v_st + hk * p.v_sh + pc));
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int wa_check(const DttWattn* g, WaP& p, const char* what) {
+    DTT_CHECK(g->dtype == 0 || g->dtype == 1, "%s: dtype must be 0 (float32) or 1 (bfloat16)", what);
+    DTT_CHECK(g->B > 0 && g->Tq > 0 && g->Tk > 0 && g->Hk > 0 && g->Hq > 0 && g->Hq % g->Hk == 0,
+              "%s: bad sizes B=%d Tq=%d Tk=%d Hq=%d Hk=%d (Hq a multiple of Hk)", what, g->B, g->Tq, g->Tk, g->Hq, g->Hk);
+    DTT_CHECK(g->DH == 32 || g->DH == 64 || g->DH == 96 || g->DH == 128, "%s: head width %d (32, 64, 96 or 128)", what, g->DH);
+    DTT_CHECK(g->left >= 0 && g->right >= 0 && g->offset >= 0 && g->left < (1 << 29) && g->right < (1 << 29) && g->offset < (1 << 29) &&
+              g->Tq < (1 << 29) && g->Tk < (1 << 29), "%s: window, offset and lengths must be in [0, 2^29)", what);
+    DTT_CHECK(g->sinks >= 0 && g->sinks <= KM, "%s: sinks=%d (0 to %d)", what, g->sinks, KM);
+    DTT_CHECK(g->scale > 0.f && g->scale < INFINITY, "%s: scale=%g must be positive", what, g->scale);
+    DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
+    const int epp = g->dtype ? 8 : 4;
+    DTT_CHECK((g->q_sb | g->q_st | g->q_sh | g->k_sb | g->k_st | g->k_sh | g->v_sb | g->v_st | g->v_sh) % epp == 0 && aligned16(g->q) &&
+              aligned16(g->k) && aligned16(g->v), "%s: rows must start on 16 bytes", what);
+    p = WaP{};
+    p.q = g->q; p.k = g->k; p.v = g->v; p.o = g->out; p.out = g->out; p.dout = g->dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
+    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
+    p.q_sb = g->q_sb; p.q_st = g->q_st; p.q_sh = g->q_sh;
+    p.k_sb = g->k_sb; p.k_st = g->k_st; p.k_sh = g->k_sh;
+    p.v_sb = g->v_sb; p.v_st = g->v_st; p.v_sh = g->v_sh;
+    p.g_sb = g->g_sb; p.g_st = g->g_st; p.g_sh = g->g_sh;
+    p.B = g->B; p.Tq = g->Tq; p.Tk = g->Tk; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk;
+    p.left = g->left; p.right = g->right; p.sinks = g->sinks < g->Tk ? g->sinks : g->Tk; p.offset = g->offset; p.scale = g->scale;
+    return 0;
+}
+
+// chunks of the rows beyond tile 0's window that see the first tokens
+void far_chunks(WaP& p) {
+    const int64_t edge = (int64_t)KM + p.left - p.offset, far = p.Tq - (edge > 0 ? edge : 0);
+    p.nchunk = 0;
+    p.chunk = 512;
+    if (p.sinks > 0 && far > 0) p.nchunk = (int)((far + p.chunk - 1) / p.chunk);
+    p.npart = 1 + 2 * p.nchunk;
+}
+int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk * p.npart * p.sinks * 2 * dh * 4 : 0; }
+
+#define WA_DH(FN, T)                                                              \
+    do {                                                                          \
+        if (g->DH == 32) FN(T, 32);                                               \
+        else if (g->DH == 64) FN(T, 64);                                          \
+        else if (g->DH == 96) FN(T, 96);                                          \
+        else FN(T, 128);                                                          \
+    } while (0)
+#define WA_DISPATCH(FN) do { if (g->dtype) WA_DH(FN, bf16); else WA_DH(FN, float); } while (0)
+}  // namespace
+
+extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
+    DTT_CHECK(g, "dtt_wattn_fwd: null argument");
+    WaP p;
+    if (int rc = wa_check(g, p, "dtt_wattn_fwd")) return rc;
+    DTT_CHECK(g->out && aligned16(g->out), "dtt_wattn_fwd: null or unaligned output");
+    p.nt = (p.Tq + BM - 1) / BM;
+    const int64_t grid = (int64_t)p.B * p.Hq * p.nt;
+    DTT_CHECK(grid < (1ll << 31), "dtt_wattn_fwd: too many rows");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define FWD(T, D) hipLaunchKernelGGL((wattn_fwd_kernel<T, D>), dim3((unsigned)grid), dim3(NTH), 0, s, p)
+    WA_DISPATCH(FWD);
+#undef FWD
+    DTT_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int64_t dtt_wattn_bwd_ws_bytes(const DttWattn* g) {
+    WaP p;
+    if (!g || wa_check(g, p, "dtt_wattn_bwd_ws_bytes")) return 0;
+    far_chunks(p);
+    return part_bytes(p, g->DH);
+}
+
+extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
+    DTT_CHECK(g, "dtt_wattn_bwd: null argument");
+    WaP p;
+    if (int rc = wa_check(g, p, "dtt_wattn_bwd")) return rc;
+    DTT_CHECK(g->out && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
+    DTT_CHECK((g->g_sb | g->g_st | g->g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
+              aligned16(g->dk) && aligned16(g->dv), "dtt_wattn_bwd: rows must start on 16 bytes");
+    far_chunks(p);
+    const int64_t need = part_bytes(p, g->DH);
+    DTT_CHECK(need == 0 || (g->ws && aligned16(g->ws) && g->ws_bytes >= need), "dtt_wattn_bwd: workspace of %lld bytes, %lld given",
+              (long long)need, (long long)g->ws_bytes);
+    p.part = (float*)g->ws;
+    p.nt = (p.Tq + BM - 1) / BM;
+    WaP pk = p;
+    pk.nt = (p.Tk + KM - 1) / KM;
+    const int64_t gq = (int64_t)p.B * p.Hq * p.nt, gk = (int64_t)p.B * p.Hk * pk.nt;
+    const int64_t gf = (int64_t)p.B * p.Hk * p.nchunk * ((p.sinks + 31) / 32), n = (int64_t)p.B * p.Hk * p.sinks * 2 * g->DH;
+    DTT_CHECK(gq < (1ll << 31) && gk + gf < (1ll << 31), "dtt_wattn_bwd: too many rows");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define BWD(T, D)                                                                                                    \
+    do {                                                                                                             \
+        hipLaunchKernelGGL((wattn_dq_kernel<T, D>), dim3((unsigned)gq), dim3(NTH), 0, s, p);                         \
+        hipLaunchKernelGGL((wattn_dkv_kernel<T, D>), dim3((unsigned)(gk + gf)), dim3(NTH), 0, s, pk, (int)gk);       \
+        if (p.nchunk)                                                                                                \
+            hipLaunchKernelGGL((wattn_sink_sum_kernel<T>), dim3((unsigned)((n + NTH - 1) / NTH)), dim3(NTH), 0, s, p, g->DH, n); \
+    } while (0)
+    WA_DISPATCH(BWD);
+#undef BWD
+    DTT_LAUNCH_CHECK();
+    return 0;
+}
+
+namespace {
+int ws_check(const DttWattnStep* g, WsP& p, const char* what) {
+    DTT_CHECK(g->dtype == 0 || g->dtype == 1, "%s: dtype must be 0 (float32) or 1 (bfloat16)", what);
+    DTT_CHECK(g->B > 0 && g->Hk > 0 && g->Hq > 0 && g->Hq % g->Hk == 0 && g->S >= 0 && g->W > 0 && (int64_t)g->S + g->W < (1 << 30),
+              "%s: bad sizes B=%d Hq=%d Hk=%d sinks=%d window=%d", what, g->B, g->Hq, g->Hk, g->S, g->W);
+    DTT_CHECK(g->DH == 32 || g->DH == 64 || g->DH == 96 || g->DH == 128, "%s: head width %d (32, 64, 96 or 128)", what, g->DH);
+    DTT_CHECK(g->scale > 0.f && g->scale < INFINITY, "%s: scale=%g must be positive", what, g->scale);
+    DTT_CHECK(g->k && g->v && g->kc && g->vc, "%s: null buffer", what);
+    const int epp = g->dtype ? 8 : 4;
+    DTT_CHECK((g->q_sb | g->q_sh | g->k_sb | g->k_st | g->k_sh | g->v_sb | g->v_st | g->v_sh | g->kc_sb | g->kc_st | g->kc_sh | g->vc_sb |
+               g->vc_st | g->vc_sh) % epp == 0 && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(g->kc) && aligned16(g->vc),
+              "%s: rows must start on 16 bytes", what);
+    p = WsP{};
+    p.q = g->q; p.k = g->k; p.v = g->v; p.kc = g->kc; p.vc = g->vc; p.out = g->out; p.pos = g->positions;
+    p.q_sb = g->q_sb; p.q_sh = g->q_sh; p.k_sb = g->k_sb; p.k_sh = g->k_sh; p.v_sb = g->v_sb; p.v_sh = g->v_sh;
+    p.kc_sb = g->kc_sb; p.kc_st = g->kc_st; p.kc_sh = g->kc_sh; p.vc_sb = g->vc_sb; p.vc_st = g->vc_st; p.vc_sh = g->vc_sh;
+    p.B = g->B; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk; p.ngrp = (p.G + 31) / 32; p.S = g->S; p.W = g->W; p.scale = g->scale;
+    // splits of the slots: while fewer than four workgroups a CU, ranges of 512 slots at least (four tiles a wave)
+    const int M = g->S + g->W;
+    const int64_t rows = (int64_t)p.B * p.Hk * p.ngrp;
+    int64_t ns = 1024 / rows, most = (M + 511) / 512;
+    ns = ns < 1 ? 1 : ns > most ? most : ns;
+    p.per = (int)(((M + ns - 1) / ns + 127) / 128 * 128);
+    p.nsplit = (M + p.per - 1) / p.per;
+    return 0;
+}
+int64_t step_bytes(const WsP& p, int dh) { return p.nsplit > 1 ? (int64_t)p.B * p.Hk * p.ngrp * p.nsplit * 32 * (dh + 2) * 4 : 0; }
+}  // namespace
+
+extern "C" int64_t dtt_wattn_step_ws_bytes(const DttWattnStep* g) {
+    WsP p;
+    if (!g || ws_check(g, p, "dtt_wattn_step_ws_bytes")) return 0;
+    return step_bytes(p, g->DH);
+}
+
+extern "C" int dtt_wattn_step(const DttWattnStep* g, void* stream) {
+    DTT_CHECK(g, "dtt_wattn_step: null argument");
+    WsP p;
+    if (int rc = ws_check(g, p, "dtt_wattn_step")) return rc;
+    DTT_CHECK(g->q && g->out && g->positions, "dtt_wattn_step: null buffer");
+    const int64_t need = step_bytes(p, g->DH);
+    DTT_CHECK(need == 0 || (g->ws && g->ws_bytes >= need), "dtt_wattn_step: workspace of %lld bytes, %lld given", (long long)need,
+              (long long)g->ws_bytes);
+    p.part = (float*)g->ws;
+    const int64_t grid = (int64_t)p.B * p.Hk * p.ngrp * p.nsplit, n = (int64_t)p.B * p.Hq * g->DH;
+    DTT_CHECK(grid < (1ll << 31) && n < (1ll << 38), "dtt_wattn_step: too many rows");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define STEP(T, D) hipLaunchKernelGGL((wattn_step_kernel<T, D>), dim3((unsigned)grid), dim3(NTH), 0, s, p)
+    WA_DISPATCH(STEP);
+#undef STEP
+    if (p.nsplit > 1) {
+        const dim3 gj((unsigned)((n + NTH - 1) / NTH));
+        if (g->dtype) hipLaunchKernelGGL((wattn_step_join_kernel<bf16>), gj, dim3(NTH), 0, s, p, g->DH);
+        else hipLaunchKernelGGL((wattn_step_join_kernel<float>), gj, dim3(NTH), 0, s, p, g->DH);
+    }
+    DTT_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int dtt_wattn_cache_fill(const DttWattnStep* g, const int32_t* lengths, int Tn, void* stream) {
+    DTT_CHECK(g, "dtt_wattn_cache_fill: null argument");
+    WsP p;
+    if (int rc = ws_check(g, p, "dtt_wattn_cache_fill")) return rc;
+    DTT_CHECK(Tn > 0, "dtt_wattn_cache_fill: T=%d", Tn);
+    const int np = g->DH / (g->dtype ? 8 : 4);
+    const int64_t n = (int64_t)p.B * (p.S + p.W) * p.Hk * np, grid = (n + NTH - 1) / NTH;
+    DTT_CHECK(grid < (1ll << 31), "dtt_wattn_cache_fill: too many rows");
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (g->dtype) hipLaunchKernelGGL((wattn_fill_kernel<bf16>), dim3((unsigned)grid), dim3(NTH), 0, s, p, lengths, Tn, g->k_st, g->v_st, np, n);
+    else hipLaunchKernelGGL((wattn_fill_kernel<float>), dim3((unsigned)grid), dim3(NTH), 0, s, p, lengths, Tn, g->k_st, g->v_st, np, n);
+    DTT_LAUNCH_CHECK();
+    return 0;
+}

@@ -12,5 +12,7 @@ from .optim import ClipAdamW  # noqa: F401
 from .io import (load_reference_checkpoint, save_reference_checkpoint, align_state_dict_keys,  # noqa: F401
                  write_wav_float32, save_separated)
 from .feeder import collate_on_device, spec_augment_on_device  # noqa: F401
+from .seqmix import (gated_recurrence, gated_recurrence_step, window_attention, window_attention_step,  # noqa: F401
+                     window_cache_fill, rotary, rotary_frequencies)
 from .graph import GraphedTrainStep  # noqa: F401
 from .dist import GradBucketReducer, ShardedClipAdamW, LocalGrads  # noqa: F401

@@ -32,6 +32,8 @@ def lib():
         _lib.dtt_gemm_ws_bytes.restype = C.c_int64
         _lib.dtt_conv3x3_wgrad_ws_bytes.restype = C.c_int64
         _lib.dtt_multi_pack_nchunks.restype = C.c_int64
+        for name in ("dtt_recurrence_ws_bytes", "dtt_recurrence_states", "dtt_wattn_bwd_ws_bytes", "dtt_wattn_step_ws_bytes"):
+            getattr(_lib, name).restype = C.c_int64
     return _lib
 
 
@@ -87,6 +89,33 @@ class DttGemm(C.Structure):
         ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
         ("cKW", C.c_int32), ("cPadF", C.c_int32), ("cPadT", C.c_int32), ("reserved2_", C.c_int32),
     ]
+
+
+def _fields(ptrs=(), i64=(), i32=(), f32=()):
+    return ([(n, C.c_void_p) for n in ptrs] + [(n, C.c_int64) for n in i64] + [(n, C.c_int32) for n in i32] +
+            [(n, C.c_float) for n in f32])
+
+
+class DttRecurrence(C.Structure):
+    _fields_ = _fields("x f dy y dx df h0 dlast last dh0 states lengths ws".split(),
+                       "ws_bytes x_so x_si x_sl f_so f_si f_sl g_so g_si g_sl".split(), "N NI L D reverse dtype".split())
+
+
+class DttRotary(C.Structure):
+    _fields_ = _fields("q k qo ko positions freq".split(), "q_sb q_st q_sh k_sb k_st k_sh p_sb p_st".split(),
+                       "B T Hq Hk dh r interleaved back pos64 dtype".split(), ("amplitude",)) + [("reserved_", C.c_int32)]
+
+
+class DttWattn(C.Structure):
+    _fields_ = _fields("q k v out lse dout dq dk dv dd lengths ws".split(),
+                       "ws_bytes q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh g_sb g_st g_sh".split(),
+                       "B Tq Tk Hq Hk DH left right sinks offset dtype".split(), ("scale",))
+
+
+class DttWattnStep(C.Structure):
+    _fields_ = _fields("q k v kc vc out positions ws".split(),
+                       "ws_bytes q_sb q_sh k_sb k_st k_sh v_sb v_st v_sh kc_sb kc_st kc_sh vc_sb vc_st vc_sh".split(),
+                       "B Hq Hk DH S W dtype".split(), ("scale",))
 
 
 def gemm_raw(**kw):
