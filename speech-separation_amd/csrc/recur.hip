@@ -446,7 +446,10 @@ Plan plan_of(int64_t N, int L, int D, bool wide) {
 // VEC = 4 needs every row of every operand on a 4-element boundary
 bool is_wide(const DttRecurrence* g) {
     const int e = g->dtype ? 2 : 4;
-    const int64_t s = g->x_so | g->x_si | g->x_sl | g->f_so | g->f_si | g->f_sl | g->g_so | g->g_si | g->g_sl | g->D;
+    int64_t s = g->D;                             // (strides of axes of one element do not count)
+    if (g->N > g->NI) s |= g->x_so | g->f_so | g->g_so;
+    if (g->NI > 1) s |= g->x_si | g->f_si | g->g_si;
+    if (g->L > 1) s |= g->x_sl | g->f_sl | g->g_sl;
     const uintptr_t a = (uintptr_t)g->x | (uintptr_t)g->f | (uintptr_t)g->dy | (uintptr_t)g->y | (uintptr_t)g->dx | (uintptr_t)g->df;
     return s % 4 == 0 && a % (4 * e) == 0;
 }

@@ -92,8 +92,9 @@ extern "C" int dtt_rotary(const DttRotary* g, void* stream) {
     DTT_CHECK(g->q && g->qo && g->positions && g->freq && (g->Hk == 0 || (g->k && g->ko)), "dtt_rotary: null buffer");
     RotP p{};
     p.x[0] = g->q; p.x[1] = g->k; p.y[0] = g->qo; p.y[1] = g->ko;
-    p.sb[0] = g->q_sb; p.st[0] = g->q_st; p.sh[0] = g->q_sh;
-    p.sb[1] = g->k_sb; p.st[1] = g->k_st; p.sh[1] = g->k_sh;
+    // (strides of axes of one element do not count)
+    p.sb[0] = g->B > 1 ? g->q_sb : 0; p.st[0] = g->T > 1 ? g->q_st : 0; p.sh[0] = g->Hq > 1 ? g->q_sh : 0;
+    p.sb[1] = g->B > 1 ? g->k_sb : 0; p.st[1] = g->T > 1 ? g->k_st : 0; p.sh[1] = g->Hk > 1 ? g->k_sh : 0;
     p.H[0] = g->Hq; p.H[1] = g->Hk;
     p.pos = g->positions; p.freq = g->freq; p.pb = g->p_sb; p.pt = g->p_st; p.pos64 = g->pos64;
     p.T = g->T; p.dh = g->dh; p.r = g->r; p.n = (int64_t)g->B * g->T;

@@ -684,16 +684,17 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     DTT_CHECK(g->sinks >= 0 && g->sinks <= KM, "%s: sinks=%d (0 to %d)", what, g->sinks, KM);
     DTT_CHECK(g->scale > 0.f && g->scale < INFINITY, "%s: scale=%g must be positive", what, g->scale);
     DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
-    const int epp = g->dtype ? 8 : 4;
-    DTT_CHECK((g->q_sb | g->q_st | g->q_sh | g->k_sb | g->k_st | g->k_sh | g->v_sb | g->v_st | g->v_sh) % epp == 0 && aligned16(g->q) &&
-              aligned16(g->k) && aligned16(g->v), "%s: rows must start on 16 bytes", what);
     p = WaP{};
     p.q = g->q; p.k = g->k; p.v = g->v; p.o = g->out; p.out = g->out; p.dout = g->dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
     p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
-    p.q_sb = g->q_sb; p.q_st = g->q_st; p.q_sh = g->q_sh;
-    p.k_sb = g->k_sb; p.k_st = g->k_st; p.k_sh = g->k_sh;
-    p.v_sb = g->v_sb; p.v_st = g->v_st; p.v_sh = g->v_sh;
-    p.g_sb = g->g_sb; p.g_st = g->g_st; p.g_sh = g->g_sh;
+    // (strides of axes of one element do not count)
+    const bool b = g->B > 1, tq = g->Tq > 1, tk = g->Tk > 1, hq = g->Hq > 1, hk = g->Hk > 1;
+    p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : 0; p.q_sh = hq ? g->q_sh : 0;
+    p.k_sb = b ? g->k_sb : 0; p.k_st = tk ? g->k_st : 0; p.k_sh = hk ? g->k_sh : 0;
+    p.v_sb = b ? g->v_sb : 0; p.v_st = tk ? g->v_st : 0; p.v_sh = hk ? g->v_sh : 0;
+    p.g_sb = b ? g->g_sb : 0; p.g_st = tq ? g->g_st : 0; p.g_sh = hq ? g->g_sh : 0;
+    DTT_CHECK((p.q_sb | p.q_st | p.q_sh | p.k_sb | p.k_st | p.k_sh | p.v_sb | p.v_st | p.v_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->q) &&
+              aligned16(g->k) && aligned16(g->v), "%s: rows must start on 16 bytes", what);
     p.B = g->B; p.Tq = g->Tq; p.Tk = g->Tk; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk;
     p.left = g->left; p.right = g->right; p.sinks = g->sinks < g->Tk ? g->sinks : g->Tk; p.offset = g->offset; p.scale = g->scale;
     return 0;
@@ -747,7 +748,7 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_bwd")) return rc;
     DTT_CHECK(g->out && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
-    DTT_CHECK((g->g_sb | g->g_st | g->g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
+    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
               aligned16(g->dk) && aligned16(g->dv), "dtt_wattn_bwd: rows must start on 16 bytes");
     far_chunks(p);
     const int64_t need = part_bytes(p, g->DH);
@@ -782,14 +783,16 @@ int ws_check(const DttWattnStep* g, WsP& p, const char* what) {
     DTT_CHECK(g->DH == 32 || g->DH == 64 || g->DH == 96 || g->DH == 128, "%s: head width %d (32, 64, 96 or 128)", what, g->DH);
     DTT_CHECK(g->scale > 0.f && g->scale < INFINITY, "%s: scale=%g must be positive", what, g->scale);
     DTT_CHECK(g->k && g->v && g->kc && g->vc, "%s: null buffer", what);
-    const int epp = g->dtype ? 8 : 4;
-    DTT_CHECK((g->q_sb | g->q_sh | g->k_sb | g->k_st | g->k_sh | g->v_sb | g->v_st | g->v_sh | g->kc_sb | g->kc_st | g->kc_sh | g->vc_sb |
-               g->vc_st | g->vc_sh) % epp == 0 && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(g->kc) && aligned16(g->vc),
-              "%s: rows must start on 16 bytes", what);
     p = WsP{};
     p.q = g->q; p.k = g->k; p.v = g->v; p.kc = g->kc; p.vc = g->vc; p.out = g->out; p.pos = g->positions;
-    p.q_sb = g->q_sb; p.q_sh = g->q_sh; p.k_sb = g->k_sb; p.k_sh = g->k_sh; p.v_sb = g->v_sb; p.v_sh = g->v_sh;
-    p.kc_sb = g->kc_sb; p.kc_st = g->kc_st; p.kc_sh = g->kc_sh; p.vc_sb = g->vc_sb; p.vc_st = g->vc_st; p.vc_sh = g->vc_sh;
+    const bool b = g->B > 1, hq = g->Hq > 1, hk = g->Hk > 1, m = g->S + g->W > 1;
+    p.q_sb = b ? g->q_sb : 0; p.q_sh = hq ? g->q_sh : 0;
+    p.k_sb = b ? g->k_sb : 0; p.k_sh = hk ? g->k_sh : 0; p.v_sb = b ? g->v_sb : 0; p.v_sh = hk ? g->v_sh : 0;
+    p.kc_sb = b ? g->kc_sb : 0; p.kc_st = m ? g->kc_st : 0; p.kc_sh = hk ? g->kc_sh : 0;
+    p.vc_sb = b ? g->vc_sb : 0; p.vc_st = m ? g->vc_st : 0; p.vc_sh = hk ? g->vc_sh : 0;
+    DTT_CHECK((p.q_sb | p.q_sh | p.k_sb | p.k_sh | p.v_sb | p.v_sh | p.kc_sb | p.kc_st | p.kc_sh | p.vc_sb | p.vc_st | p.vc_sh) %
+              (g->dtype ? 8 : 4) == 0 && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(g->kc) && aligned16(g->vc),
+              "%s: rows must start on 16 bytes", what);
     p.B = g->B; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk; p.ngrp = (p.G + 31) / 32; p.S = g->S; p.W = g->W; p.scale = g->scale;
     // splits of the slots: while fewer than four workgroups a CU, ranges of 512 slots at least (four tiles a wave)
     const int M = g->S + g->W;
@@ -838,6 +841,7 @@ extern "C" int dtt_wattn_cache_fill(const DttWattnStep* g, const int32_t* length
     WsP p;
     if (int rc = ws_check(g, p, "dtt_wattn_cache_fill")) return rc;
     DTT_CHECK(Tn > 0, "dtt_wattn_cache_fill: T=%d", Tn);
+    DTT_CHECK(Tn == 1 || (g->k_st | g->v_st) % (g->dtype ? 8 : 4) == 0, "dtt_wattn_cache_fill: rows must start on 16 bytes");
     const int np = g->DH / (g->dtype ? 8 : 4);
     const int64_t n = (int64_t)p.B * (p.S + p.W) * p.Hk * np, grid = (n + NTH - 1) / NTH;
     DTT_CHECK(grid < (1ll << 31), "dtt_wattn_cache_fill: too many rows");

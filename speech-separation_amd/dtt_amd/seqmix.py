@@ -20,122 +20,111 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import lib, check, stream_ptr, dtype_code, DttError, DttRecurrence, DttRotary, DttWattn, DttWattnStep
 
-F32 = torch.float32
+# The single-frame forms and short training steps are bound by what the host spends on a call: arguments are checked with
+# plain comparisons (messages are formatted on failure alone), structs are filled once and kept for the backward call.
+
+F32, BF16, F64, I32, I64 = torch.float32, torch.bfloat16, torch.float64, torch.int32, torch.int64
+_device = torch._C._cuda_getDevice
 
 
 # --------------------------------------------------------------------------- #
 # arguments
 # --------------------------------------------------------------------------- #
-class _on:
-    """Launches inside go to `dev`, whatever the current device is."""
-
-    def __init__(self, dev):
-        self.ctx = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+def _fail(name, what):
+    raise DttError(f"{name}: {what}")
 
 
-def _need(ok, what):
-    if not ok:
-        raise DttError(what)
+def _on_gpu(name, t):
+    if not t.is_cuda:
+        _fail(name, "dtt_amd ops need CUDA(HIP) tensors; there is no CPU path")
+    if t.dtype is not F32 and t.dtype is not BF16:
+        dtype_code(t.dtype)
 
 
-def _same(name, first, *others):
-    """`others` ((name, tensor) pairs, None allowed) on first's device; first on a GPU."""
-    if not first.is_cuda:
-        raise DttError("dtt_amd ops need CUDA(HIP) tensors; there is no CPU path")
-    for n, t in others:
-        if t is not None and t.device != first.device:
-            raise DttError(f"{name}: {n} is on {t.device}, the other tensors on {first.device}")
+def _beside(name, t, what, other):
+    if other.device != t.device:
+        _fail(name, f"{what} is on {other.device}, the other tensors on {t.device}")
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+def _inner(t):
+    """`t` with a contiguous innermost axis, a copy if it has not."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _rows(t, bytes_=1):
-    """`t` with a contiguous innermost axis and, where asked, every row on `bytes_` bytes; a copy if it has not."""
-    e = t.element_size()
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (bytes_ <= e or (
-            t.data_ptr() % bytes_ == 0 and all(s * e % bytes_ == 0 or n == 1 for s, n in zip(t.stride()[:-1], t.shape)))):
-        return t
+def _rows16(t):
+    """`t` with a contiguous innermost axis and every row on 16 bytes, a copy if it has not."""
+    st, e = t.stride(), t.element_size()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        bits = 0
+        for s in st[:-1]:
+            bits |= s
+        if bits * e % 16 == 0 or all(s * e % 16 == 0 or n == 1 for s, n in zip(st[:-1], t.shape)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _strides(t):
-    """Strides of all axes but the innermost; 0 for axes of one element."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
 
 
 def _lengths(name, lengths, batch, first):
     if lengths is None:
         return None
-    _need(torch.is_tensor(lengths) and lengths.dtype in (torch.int32, torch.int64) and tuple(lengths.shape) == tuple(batch),
-          f"{name}: lengths must be an int32 or int64 tensor of shape {tuple(batch)}")
-    _same(name, first, ("lengths", lengths))
-    return lengths.to(torch.int32).contiguous()
+    if not torch.is_tensor(lengths) or lengths.dtype not in (I32, I64) or lengths.shape != batch:
+        _fail(name, f"lengths must be an int32 or int64 tensor of shape {tuple(batch)}")
+    _beside(name, first, "lengths", lengths)
+    # (int64 lengths are clamped into int32 rather than wrapped: C treats all beyond the sequence alike)
+    return (lengths if lengths.dtype is I32 else lengths.clamp(-1, (1 << 31) - 1).to(I32)).contiguous()
 
 
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _workspace(g, need, dev):
+    """Scratch for one call; the caller keeps the tensor until the call is enqueued (the caching allocator orders reuse)."""
+    if need <= 0:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    g.ws, g.ws_bytes = ws.data_ptr(), need
+    return ws
 
 
-def _workspace(n, dev):
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
+def _again(g):
+    """A copy of a forward call's struct: backward calls of one graph may run at the same time."""
+    return type(g).from_buffer_copy(g)
 
 
 # --------------------------------------------------------------------------- #
 # gated linear recurrence
 # --------------------------------------------------------------------------- #
-def _rec_args(x, f, reverse, lengths, h0):
-    """The struct's common part; x, f [(outer,) inner, L, D] as rows."""
-    L, D = x.shape[-2:]
-    n = x.numel() // (L * D)
-    ni = x.shape[1] if x.dim() == 4 else 1
-    g = DttRecurrence(N=n, NI=ni, L=L, D=D, reverse=1 if reverse else 0, dtype=dtype_code(x.dtype))
-    g.x, g.f, g.lengths, g.h0 = x.data_ptr(), f.data_ptr(), _p(lengths), _p(h0)
-    g.x_so, g.x_si, g.x_sl = _rec_strides(x)
-    g.f_so, g.f_si, g.f_sl = _rec_strides(f)
-    return g
-
-
 def _rec_strides(t):
-    s = _strides(t)
-    return s if len(s) == 3 else (s[0], 0, s[1])
+    s = t.stride()
+    return s[:3] if len(s) == 4 else (s[0], 0, s[1])
 
 
 def _rec_forward(x, f, h0, reverse, lengths, keep):
-    dev = x.device
-    with _on(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        last = torch.empty(x.shape[:-2] + x.shape[-1:], dtype=F32, device=dev)
-        g = _rec_args(x, f, reverse, lengths, h0)
-        g.y, g.last = y.data_ptr(), last.data_ptr()
-        L = lib()
-        states = None
-        if keep:
-            states = torch.empty(L.dtt_recurrence_states(C.byref(g)), dtype=F32, device=dev)
-            g.states = states.data_ptr()
-        ws = _workspace(L.dtt_recurrence_ws_bytes(C.byref(g)), dev)
-        if ws is not None:
-            g.ws, g.ws_bytes = ws.data_ptr(), ws.numel()
-        check(L.dtt_recurrence_fwd(C.byref(g), stream_ptr()), "dtt_recurrence_fwd")
-    return y, last, states
+    shape = x.shape
+    L, D = shape[-2:]
+    N = math.prod(shape[:-2])
+    g = DttRecurrence(N=N, NI=shape[1] if len(shape) == 4 else 1, L=L, D=D, reverse=1 if reverse else 0,
+                      dtype=1 if x.dtype is BF16 else 0)
+    g.x, g.f = x.data_ptr(), f.data_ptr()
+    g.x_so, g.x_si, g.x_sl = _rec_strides(x)
+    g.f_so, g.f_si, g.f_sl = _rec_strides(f)
+    if lengths is not None:
+        g.lengths = lengths.data_ptr()
+    if h0 is not None:
+        g.h0 = h0.data_ptr()
+    y = x.new_empty(shape)
+    last = torch.empty(shape[:-2] + shape[-1:], dtype=F32, device=x.device)
+    g.y, g.last = y.data_ptr(), last.data_ptr()
+    lib_, ref, states = lib(), C.byref(g), None
+    if keep:
+        states = torch.empty(lib_.dtt_recurrence_states(ref), dtype=F32, device=x.device)
+        g.states = states.data_ptr()
+    ws = _workspace(g, lib_.dtt_recurrence_ws_bytes(ref), x.device)  # noqa: F841 (alive until the call returns)
+    check(lib_.dtt_recurrence_fwd(ref, stream_ptr()), "dtt_recurrence_fwd")
+    return y, last, states, g
 
 
 class GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, h0, reverse, lengths):
-        y, last, states = _rec_forward(x, f, h0, reverse, lengths, True)
+        y, last, states, ctx.call = _rec_forward(x, f, h0, reverse, lengths, True)
         ctx.save_for_backward(x, f, h0, lengths, states)
-        ctx.reverse = reverse
         ctx.set_materialize_grads(False)
         return y, last
 
@@ -143,21 +132,20 @@ class GatedRecurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dlast):
         x, f, h0, lengths, states = ctx.saved_tensors
-        dev = x.device
-        with _on(dev):
-            dy = torch.zeros(x.shape[-1], dtype=x.dtype, device=dev).expand(x.shape) if dy is None else _rows(dy)
-            dlast = dlast.contiguous() if dlast is not None else None
-            dx, df = (torch.empty(x.shape, dtype=x.dtype, device=dev) for _ in range(2))
-            dh0 = torch.empty(h0.shape, dtype=F32, device=dev) if h0 is not None and ctx.needs_input_grad[2] else None
-            g = _rec_args(x, f, ctx.reverse, lengths, h0)
-            g.dy, g.dx, g.df, g.dlast, g.dh0, g.states = (dy.data_ptr(), dx.data_ptr(), df.data_ptr(), _p(dlast), _p(dh0),
-                                                         states.data_ptr())
-            g.g_so, g.g_si, g.g_sl = _rec_strides(dy)
-            L = lib()
-            ws = _workspace(L.dtt_recurrence_ws_bytes(C.byref(g)), dev)
-            if ws is not None:
-                g.ws, g.ws_bytes = ws.data_ptr(), ws.numel()
-            check(L.dtt_recurrence_bwd(C.byref(g), stream_ptr()), "dtt_recurrence_bwd")
+        g = _again(ctx.call)
+        dy = x.new_zeros(x.shape[-1]).expand(x.shape) if dy is None else _inner(dy)
+        if dlast is not None:
+            dlast = dlast.contiguous()
+            g.dlast = dlast.data_ptr()
+        dx, df, dh0 = x.new_empty(x.shape), x.new_empty(x.shape), None
+        if h0 is not None and ctx.needs_input_grad[2]:
+            dh0 = torch.empty_like(h0)
+            g.dh0 = dh0.data_ptr()
+        g.dy, g.dx, g.df = dy.data_ptr(), dx.data_ptr(), df.data_ptr()
+        g.g_so, g.g_si, g.g_sl = _rec_strides(dy)
+        lib_, ref = lib(), C.byref(g)
+        ws = _workspace(g, lib_.dtt_recurrence_ws_bytes(ref), x.device)  # noqa: F841
+        check(lib_.dtt_recurrence_bwd(ref, stream_ptr()), "dtt_recurrence_bwd")
         return dx, df, dh0, None, None
 
 
@@ -170,20 +158,29 @@ def gated_recurrence(x, f, h0=None, reverse=False, lengths=None):
     from lengths on are padding: never read, y and the gradients are 0 there, and ``last`` is the state of the item's own
     last step.  Differentiable in x, f and h0; states are float32 throughout."""
     name = "gated_recurrence"
-    _need(torch.is_tensor(x) and torch.is_tensor(f) and x.dim() in (3, 4) and x.shape == f.shape,
-          f"{name}: x and f must have one shape, [B, L, D] or [B, N, L, D]")
-    _same(name, x, ("f", f), ("h0", h0))
-    _need(x.dtype == f.dtype, f"{name}: x is {x.dtype}, f is {f.dtype}")
-    dtype_code(x.dtype)
-    batch, D = x.shape[:-2], x.shape[-1]
+    if not torch.is_tensor(x) or not torch.is_tensor(f) or x.dim() not in (3, 4) or x.shape != f.shape:
+        _fail(name, "x and f must have one shape, [B, L, D] or [B, N, L, D]")
+    _on_gpu(name, x)
+    if x.dtype is not f.dtype:
+        _fail(name, f"x is {x.dtype}, f is {f.dtype}")
+    _beside(name, x, "f", f)
+    batch = x.shape[:-2]
     if h0 is not None:
-        _need(h0.dtype == F32 and tuple(h0.shape) == tuple(batch) + (D,), f"{name}: h0 must be float32 {tuple(batch) + (D,)}")
-    lengths = _lengths(name, lengths, batch, x)
+        if h0.dtype is not F32 or h0.shape != batch + x.shape[-1:]:
+            _fail(name, f"h0 must be float32 {tuple(batch + x.shape[-1:])}")
+        _beside(name, x, "h0", h0)
+    if lengths is not None:
+        lengths = _lengths(name, lengths, batch, x)
     if x.numel() == 0:
-        return x * f, (h0.clone() if h0 is not None else torch.zeros(tuple(batch) + (D,), dtype=F32, device=x.device))
-    x, f, h0 = _rows(x), _rows(f), h0.contiguous() if h0 is not None else None
-    if _wants_grad(x, f, h0):
-        return GatedRecurrence.apply(x, f, h0, bool(reverse), lengths)
+        return x * f, (h0.clone() if h0 is not None else torch.zeros(batch + x.shape[-1:], dtype=F32, device=x.device))
+    if x.get_device() != _device():
+        with torch.cuda.device(x.device):
+            return gated_recurrence(x, f, h0, reverse, lengths)
+    x, f = _inner(x), _inner(f)
+    if h0 is not None:
+        h0 = h0.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or f.requires_grad or (h0 is not None and h0.requires_grad)):
+        return GatedRecurrence.apply(x, f, h0, reverse, lengths)
     return _rec_forward(x, f, h0, reverse, lengths, False)[:2]
 
 
@@ -191,89 +188,85 @@ def gated_recurrence_step(x, f, state):
     """One step of gated_recurrence for every item: x, f [N, D], state float32 [N, D] (contiguous), replaced by the new
     state; returns it in x's dtype.  No gradients."""
     name = "gated_recurrence_step"
-    _need(x.dim() == 2 and x.shape == f.shape and x.shape == state.shape, f"{name}: x, f and state must have one shape [N, D]")
-    _same(name, x, ("f", f), ("state", state))
-    _need(x.dtype == f.dtype and state.dtype == F32 and state.is_contiguous(),
-          f"{name}: x and f of one dtype, state float32 and contiguous")
-    _need(not _wants_grad(x, f, state), f"{name} has no gradient: call it under torch.no_grad()")
-    d = dtype_code(x.dtype)
+    if x.dim() != 2 or x.shape != f.shape or x.shape != state.shape:
+        _fail(name, "x, f and state must have one shape [N, D]")
+    _on_gpu(name, x)
+    if x.dtype is not f.dtype or state.dtype is not F32 or not state.is_contiguous():
+        _fail(name, "x and f must have one dtype, state must be float32 and contiguous")
+    if f.device != x.device or state.device != x.device:
+        _fail(name, "x, f and state must be on one device")
+    if torch.is_grad_enabled() and (x.requires_grad or f.requires_grad or state.requires_grad):
+        _fail(name, "no gradient: call it under torch.no_grad()")
+    if x.get_device() != _device():
+        with torch.cuda.device(x.device):
+            return gated_recurrence_step(x, f, state)
     N, D = x.shape
-    x, f = _rows(x), _rows(f)
-    y = torch.empty((N, D), dtype=x.dtype, device=x.device)
-    if y.numel():
-        with _on(x.device):
-            check(lib().dtt_recurrence_step(C.c_void_p(x.data_ptr()), C.c_void_p(f.data_ptr()), C.c_void_p(state.data_ptr()),
-                                            C.c_void_p(y.data_ptr()), N, D, C.c_int64(x.stride(0) if N > 1 else 0),
-                                            C.c_int64(f.stride(0) if N > 1 else 0), d, stream_ptr()), "dtt_recurrence_step")
+    x, f, y = _inner(x), _inner(f), torch.empty((N, D), dtype=x.dtype, device=x.device)
+    if N * D:
+        check(lib().dtt_recurrence_step(C.c_void_p(x.data_ptr()), C.c_void_p(f.data_ptr()), C.c_void_p(state.data_ptr()),
+                                        C.c_void_p(y.data_ptr()), N, D, C.c_int64(x.stride(0)), C.c_int64(f.stride(0)),
+                                        1 if x.dtype is BF16 else 0, stream_ptr()), "dtt_recurrence_step")
     return y
 
 
 # --------------------------------------------------------------------------- #
 # windowed attention
 # --------------------------------------------------------------------------- #
-def _attn_args(q, k, v, lengths, cfg):
-    left, right, sinks, offset, scale = cfg
-    B, Tq, Hq, dh = q.shape
-    g = DttWattn(B=B, Tq=Tq, Tk=k.shape[1], Hq=Hq, Hk=k.shape[2], DH=dh, left=left, right=right, sinks=sinks, offset=offset,
-                 dtype=dtype_code(q.dtype), scale=scale)
-    g.q, g.k, g.v, g.lengths = q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(lengths)
-    g.q_sb, g.q_st, g.q_sh = _strides(q)
-    g.k_sb, g.k_st, g.k_sh = _strides(k)
-    g.v_sb, g.v_st, g.v_sh = _strides(v)
-    return g
-
-
 def _attn_forward(q, k, v, lengths, cfg, keep):
-    with _on(q.device):
-        B, Tq, Hq, dh = q.shape
-        out = torch.empty((B, Tq, Hq, dh), dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, Hq, Tq), dtype=F32, device=q.device) if keep else None
-        g = _attn_args(q, k, v, lengths, cfg)
-        g.out, g.lse = out.data_ptr(), _p(lse)
-        check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
-    return out, lse
+    B, Tq, Hq, dh = q.shape
+    g = DttWattn(B=B, Tq=Tq, Tk=k.shape[1], Hq=Hq, Hk=k.shape[2], DH=dh, left=cfg[0], right=cfg[1], sinks=cfg[2], offset=cfg[3],
+                 dtype=1 if q.dtype is BF16 else 0, scale=cfg[4])
+    g.q, g.k, g.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    g.q_sb, g.q_st, g.q_sh, _ = q.stride()
+    g.k_sb, g.k_st, g.k_sh, _ = k.stride()
+    g.v_sb, g.v_st, g.v_sh, _ = v.stride()
+    if lengths is not None:
+        g.lengths = lengths.data_ptr()
+    out, lse = q.new_empty(q.shape), None
+    g.out = out.data_ptr()
+    if keep:
+        lse = torch.empty((B, Hq, Tq), dtype=F32, device=q.device)
+        g.lse = lse.data_ptr()
+    check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
+    return out, lse, g
 
 
 class WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, cfg):
-        out, lse = _attn_forward(q, k, v, lengths, cfg, True)
+        out, lse, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
         ctx.save_for_backward(q, k, v, lengths, out, lse)
-        ctx.cfg = cfg
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         q, k, v, lengths, out, lse = ctx.saved_tensors
-        dev = q.device
-        with _on(dev):
-            do = _rows(do, 16)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-            dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=dev) for _ in range(2))
-            dd = torch.empty_like(lse)
-            g = _attn_args(q, k, v, lengths, ctx.cfg)
-            g.out, g.lse, g.dout, g.dq, g.dk, g.dv, g.dd = (out.data_ptr(), lse.data_ptr(), do.data_ptr(), dq.data_ptr(),
-                                                           dk.data_ptr(), dv.data_ptr(), dd.data_ptr())
-            g.g_sb, g.g_st, g.g_sh = _strides(do)
-            L = lib()
-            ws = _workspace(L.dtt_wattn_bwd_ws_bytes(C.byref(g)), dev)
-            if ws is not None:
-                g.ws, g.ws_bytes = ws.data_ptr(), ws.numel()
-            check(L.dtt_wattn_bwd(C.byref(g), stream_ptr()), "dtt_wattn_bwd")
+        do, g = _rows16(do), _again(ctx.call)
+        dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse)
+        g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
+        g.g_sb, g.g_st, g.g_sh, _ = do.stride()
+        lib_, ref = lib(), C.byref(g)
+        ws = _workspace(g, lib_.dtt_wattn_bwd_ws_bytes(ref), q.device)  # noqa: F841 (alive until the call returns)
+        check(lib_.dtt_wattn_bwd(ref, stream_ptr()), "dtt_wattn_bwd")
         return dq, dk, dv, None, None
 
 
 def _heads_check(name, q, k, v, dims):
-    _need(all(torch.is_tensor(t) and t.dim() == dims for t in (q, k, v)), f"{name}: q, k and v must have {dims} axes")
-    _same(name, q, ("k", k), ("v", v))
-    _need(q.dtype == k.dtype == v.dtype, f"{name}: q, k and v must have one dtype")
-    dtype_code(q.dtype)
-    _need(k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[-1] == q.shape[-1],
-          f"{name}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
-    _need(k.shape[-2] > 0 and q.shape[-2] > 0 and q.shape[-2] % k.shape[-2] == 0,
-          f"{name}: {q.shape[-2]} query heads over {k.shape[-2]} key heads")
-    _need(q.shape[-1] in (32, 64, 96, 128), f"{name}: head width {q.shape[-1]} (32, 64, 96 or 128)")
+    if not (torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v)) or q.dim() != dims or k.dim() != dims:
+        _fail(name, f"q, k and v must be tensors of {dims} axes")
+    _on_gpu(name, q)
+    qs, ks = q.shape, k.shape
+    if ks != v.shape or ks[0] != qs[0] or ks[-1] != qs[-1]:
+        _fail(name, f"shapes {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)} do not fit")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+        _fail(name, "q, k and v must have one dtype")
+    if k.device != q.device or v.device != q.device:
+        _fail(name, f"q, k and v are on {q.device}, {k.device} and {v.device}")
+    if qs[-2] == 0 or ks[-2] == 0 or qs[-2] % ks[-2]:
+        _fail(name, f"{qs[-2]} query heads over {ks[-2]} key heads")
+    if qs[-1] not in (32, 64, 96, 128):
+        _fail(name, f"head width {qs[-1]} (32, 64, 96 or 128)")
 
 
 _BIG = 1 << 28
@@ -285,45 +278,48 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
 
     q [B, Tq, Hq, dh], k, v [B, Tk, Hk, dh] of one dtype, Hq a multiple of Hk (query head h reads key head
     h // (Hq // Hk)), dh 32, 64, 96 or 128; ``sinks`` <= 128.  ``offset`` defaults to Tk - Tq (the queries are the last
-    Tq positions), ``scale`` (positive) to dh ** -0.5.  ``lengths`` [B]: positions from lengths on are padding -- keys there are never
-    read, rows there are zero and take no part in any gradient.  A non-finite key or value inside lengths may reach rows
-    of the same 32 positions that do not see it.  Differentiable in q, k and v."""
+    Tq positions), ``scale`` (positive) to dh ** -0.5.  ``lengths`` [B]: positions from lengths on are padding -- keys there
+    are never read, rows there are zero and take no part in any gradient.  A non-finite key or value inside lengths may
+    reach rows of the same 32 positions that do not see it.  Differentiable in q, k and v."""
     name = "window_attention"
     _heads_check(name, q, k, v, 4)
-    B, Tq, Hq, dh = q.shape
-    Tk = k.shape[1]
+    Tq, Tk = q.shape[1], k.shape[1]
     offset = Tk - Tq if offset is None else int(offset)
     left, right, sinks = int(left), int(right), int(sinks)
-    _need(left >= 0 and right >= 0 and 0 <= sinks <= 128, f"{name}: left={left}, right={right} and sinks={sinks} (0 to 128)")
-    _need(0 <= offset < _BIG and Tq < _BIG and Tk < _BIG, f"{name}: offset={offset}, Tq={Tq}, Tk={Tk} must be in [0, 2^28)")
-    lengths = _lengths(name, lengths, (B,), q)
+    if left < 0 or right < 0 or not 0 <= sinks <= 128:
+        _fail(name, f"left={left}, right={right} and sinks={sinks} (0 to 128)")
+    if not 0 <= offset < _BIG or Tq >= _BIG or Tk >= _BIG:
+        _fail(name, f"offset={offset}, Tq={Tq}, Tk={Tk} must be in [0, 2^28)")
+    if lengths is not None:
+        lengths = _lengths(name, lengths, q.shape[:1], q)
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if q.numel() == 0 or Tk == 0:
-        return q * 0.0 + k.sum() * 0.0 + v.sum() * 0.0 if _wants_grad(q, k, v) else torch.zeros_like(q)
-    cfg = (min(left, _BIG), min(right, _BIG), sinks, offset, dh ** -0.5 if scale is None else float(scale))
-    q, k, v = _rows(q, 16), _rows(k, 16), _rows(v, 16)
-    if _wants_grad(q, k, v):
-        return WindowAttention.apply(q, k, v, lengths, cfg)
-    return _attn_forward(q, k, v, lengths, cfg, False)[0]
+        return q * 0.0 + k.sum() * 0.0 + v.sum() * 0.0 if grad else torch.zeros_like(q)
+    if q.get_device() != _device():
+        with torch.cuda.device(q.device):
+            return window_attention(q, k, v, left, right, sinks, lengths, offset, scale)
+    cfg = (min(left, _BIG), min(right, _BIG), sinks, offset, q.shape[-1] ** -0.5 if scale is None else float(scale))
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    return WindowAttention.apply(q, k, v, lengths, cfg) if grad else _attn_forward(q, k, v, lengths, cfg, False)[0]
 
 
-def _cache_check(name, k, k_cache, v_cache, sinks):
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[0] == k.shape[0] and
-          k_cache.shape[2:] == k.shape[-2:], f"{name}: caches must be [B, sinks + window, Hk, dh], got {tuple(k_cache.shape)}")
-    _need(k_cache.dtype == k.dtype and v_cache.dtype == k.dtype, f"{name}: caches must have the dtype of k")
-    _same(name, k, ("k_cache", k_cache), ("v_cache", v_cache))
-    _need(0 <= sinks < k_cache.shape[1], f"{name}: sinks={sinks} of {k_cache.shape[1]} slots (at least one for the window)")
-    for c in (k_cache, v_cache):
-        e = c.element_size()
-        _need(c.stride(-1) == 1 and c.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in c.stride()[:-1]),
-              f"{name}: cache rows must be contiguous and start on 16 bytes")
-
-
-def _step_args(k, v, k_cache, v_cache, sinks, scale):
-    B, M, Hk, dh = k_cache.shape
-    g = DttWattnStep(B=B, Hq=Hk, Hk=Hk, DH=dh, S=sinks, W=M - sinks, dtype=dtype_code(k.dtype), scale=scale)
-    g.k, g.v, g.kc, g.vc = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    g.kc_sb, g.kc_st, g.kc_sh = _strides(k_cache)
-    g.vc_sb, g.vc_st, g.vc_sh = _strides(v_cache)
+def _step_args(name, k, v, k_cache, v_cache, sinks, scale):
+    """Checks the caches of k, v and fills what the step and the fill share."""
+    cs = k_cache.shape
+    if len(cs) != 4 or cs != v_cache.shape or cs[0] != k.shape[0] or cs[2:] != k.shape[-2:]:
+        _fail(name, f"caches must be [B, sinks + window, Hk, dh], got {tuple(cs)} and {tuple(v_cache.shape)}")
+    if k_cache.dtype is not k.dtype or v_cache.dtype is not k.dtype:
+        _fail(name, "caches must have the dtype of k")
+    if k_cache.device != k.device or v_cache.device != k.device:
+        _fail(name, "caches must be on the device of k")
+    if not 0 <= sinks < cs[1]:
+        _fail(name, f"sinks={sinks} of {cs[1]} slots (at least one for the window)")
+    g = DttWattnStep(B=cs[0], Hq=cs[2], Hk=cs[2], DH=cs[3], S=sinks, W=cs[1] - sinks, dtype=1 if k.dtype is BF16 else 0, scale=scale)
+    g.kc_sb, g.kc_st, g.kc_sh, ke = k_cache.stride()
+    g.vc_sb, g.vc_st, g.vc_sh, ve = v_cache.stride()
+    g.kc, g.vc = k_cache.data_ptr(), v_cache.data_ptr()
+    if ke != 1 or ve != 1 or (g.kc | g.vc) % 16 or (g.kc_sb | g.kc_st | g.kc_sh | g.vc_sb | g.vc_st | g.vc_sh) * k.element_size() % 16:
+        _fail(name, "cache rows must be contiguous and start on 16 bytes")
     return g
 
 
@@ -335,28 +331,27 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, sinks=0, scale=N
     An item with a negative position is idle: its cache stays as it is and its row is zero.  No gradients."""
     name = "window_attention_step"
     _heads_check(name, q, k, v, 3)
-    sinks = int(sinks)
-    _cache_check(name, k, k_cache, v_cache, sinks)
-    _need(positions.dtype == torch.int64 and positions.dim() == 1 and positions.shape[0] == q.shape[0] and positions.is_contiguous(),
-          f"{name}: positions must be a contiguous int64 tensor [B]")
-    _same(name, q, ("positions", positions), ("k_cache", k_cache))
-    _need(not _wants_grad(q, k, v), f"{name} has no gradient: call it under torch.no_grad()")
+    if positions.dtype is not I64 or positions.dim() != 1 or positions.shape[0] != q.shape[0] or not positions.is_contiguous():
+        _fail(name, "positions must be a contiguous int64 tensor [B]")
+    _beside(name, q, "positions", positions)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        _fail(name, "no gradient: call it under torch.no_grad()")
+    if q.get_device() != _device():
+        with torch.cuda.device(q.device):
+            return window_attention_step(q, k, v, k_cache, v_cache, positions, sinks, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.numel() == 0:
+    if q.shape[0] == 0:
         return out
-    q, k, v = _rows(q, 16), _rows(k, 16), _rows(v, 16)
-    with _on(q.device):
-        g = _step_args(k, v, k_cache, v_cache, sinks, q.shape[-1] ** -0.5 if scale is None else float(scale))
-        g.Hq = q.shape[1]
-        g.q, g.out, g.positions = q.data_ptr(), out.data_ptr(), positions.data_ptr()
-        g.q_sb, g.q_sh = _strides(q)
-        g.k_sb, g.k_sh = _strides(k)
-        g.v_sb, g.v_sh = _strides(v)
-        L = lib()
-        ws = _workspace(L.dtt_wattn_step_ws_bytes(C.byref(g)), q.device)
-        if ws is not None:
-            g.ws, g.ws_bytes = ws.data_ptr(), ws.numel()
-        check(L.dtt_wattn_step(C.byref(g), stream_ptr()), "dtt_wattn_step")
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    g = _step_args(name, k, v, k_cache, v_cache, int(sinks), q.shape[-1] ** -0.5 if scale is None else float(scale))
+    g.Hq = q.shape[1]
+    g.q, g.k, g.v, g.out, g.positions = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), positions.data_ptr()
+    g.q_sb, g.q_sh, _ = q.stride()
+    g.k_sb, g.k_sh, _ = k.stride()
+    g.v_sb, g.v_sh, _ = v.stride()
+    lib_, ref = lib(), C.byref(g)
+    ws = _workspace(g, lib_.dtt_wattn_step_ws_bytes(ref), q.device)  # noqa: F841 (alive until the call returns)
+    check(lib_.dtt_wattn_step(ref, stream_ptr()), "dtt_wattn_step")
     return out
 
 
@@ -366,18 +361,21 @@ def window_cache_fill(k, v, k_cache, v_cache, sinks=0, lengths=None):
     those positions stay as they are."""
     name = "window_cache_fill"
     _heads_check(name, k, k, v, 4)
-    sinks = int(sinks)
-    _cache_check(name, k, k_cache, v_cache, sinks)
-    _need(k.shape[1] < _BIG, f"{name}: T={k.shape[1]}")
+    if k.shape[1] >= _BIG:
+        _fail(name, f"T={k.shape[1]} must be below 2^28")
     lengths = _lengths(name, lengths, k.shape[:1], k)
+    if k.get_device() != _device():
+        with torch.cuda.device(k.device):
+            return window_cache_fill(k, v, k_cache, v_cache, sinks, lengths)
+    k, v = _rows16(k.detach()), _rows16(v.detach())
+    g = _step_args(name, k, v, k_cache, v_cache, int(sinks), 1.0)
     if k.numel() == 0:
         return
-    k, v = _rows(k.detach(), 16), _rows(v.detach(), 16)
-    with _on(k.device):
-        g = _step_args(k, v, k_cache, v_cache, sinks, 1.0)
-        g.k_sb, g.k_st, g.k_sh = _strides(k)
-        g.v_sb, g.v_st, g.v_sh = _strides(v)
-        check(lib().dtt_wattn_cache_fill(C.byref(g), C.c_void_p(_p(lengths)), k.shape[1], stream_ptr()), "dtt_wattn_cache_fill")
+    g.k, g.v = k.data_ptr(), v.data_ptr()
+    g.k_sb, g.k_st, g.k_sh, _ = k.stride()
+    g.v_sb, g.v_st, g.v_sh, _ = v.stride()
+    check(lib().dtt_wattn_cache_fill(C.byref(g), C.c_void_p(None if lengths is None else lengths.data_ptr()), k.shape[1],
+                                     stream_ptr()), "dtt_wattn_cache_fill")
 
 
 # --------------------------------------------------------------------------- #
@@ -388,56 +386,52 @@ def rotary_frequencies(dim, base=10000.0, stretch=1.0, trained=None, blend=(1.0,
     times longer than the trained one.  With ``trained`` (that context's length) only slow pairs are stretched: a pair that
     turns ``blend[1]`` times or more over it keeps its frequency, one that turns ``blend[0]`` times or fewer is divided by
     stretch, those between are blended linearly in their number of turns."""
-    _need(dim > 0 and dim % 2 == 0 and base > 0 and stretch > 0, f"rotary_frequencies: dim={dim}, base={base}, stretch={stretch}")
-    i = torch.arange(dim // 2, dtype=torch.float64, device=device)
+    name = "rotary_frequencies"
+    if not (dim > 0 and dim % 2 == 0 and base > 0 and stretch > 0):
+        _fail(name, f"dim={dim} (even), base={base}, stretch={stretch}")
+    i = torch.arange(dim // 2, dtype=F64, device=device)
     freq = torch.exp(i * (-2.0 * math.log(base) / dim))
     if trained is None:
         return freq / stretch
     lo, hi = blend
-    _need(trained > 0 and hi > lo >= 0, f"rotary_frequencies: trained={trained}, blend={blend}")
+    if not (trained > 0 and hi > lo >= 0):
+        _fail(name, f"trained={trained}, blend={blend}")
     keep = ((trained * freq / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
     return freq * (keep + (1.0 - keep) / stretch)
 
 
-def _rotate(q, k, positions, freq, interleaved, amplitude, back):
-    """q (k: or None) [B, T, H, dh] -> turned copies."""
-    B, T, Hq, dh = q.shape
-    with _on(q.device):
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
-        g = DttRotary(B=B, T=T, Hq=Hq, Hk=k.shape[2] if k is not None else 0, dh=dh, r=2 * freq.shape[0],
-                      interleaved=1 if interleaved else 0, back=1 if back else 0, pos64=1 if positions.dtype == torch.int64 else 0,
-                      dtype=dtype_code(q.dtype), amplitude=amplitude)
-        g.q, g.k, g.qo, g.ko, g.positions, g.freq = q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), positions.data_ptr(), freq.data_ptr()
-        g.q_sb, g.q_st, g.q_sh = _strides(q)
-        if k is not None:
-            g.k_sb, g.k_st, g.k_sh = _strides(k)
-        if positions.dim() == 2:
-            g.p_sb, g.p_st = positions.stride()
-        else:
-            g.p_st = positions.stride(0)
-        check(lib().dtt_rotary(C.byref(g), stream_ptr()), "dtt_rotary")
+def _rotate(q, k, g):
+    """q and k (or None) [B, T, H, dh] -> turned copies, by the positions, frequencies and layout that `g` holds."""
+    qo, ko = q.new_empty(q.shape), None
+    g.q, g.qo, g.Hq = q.data_ptr(), qo.data_ptr(), q.shape[2]
+    g.q_sb, g.q_st, g.q_sh, _ = q.stride()
+    if k is not None:
+        ko = k.new_empty(k.shape)
+        g.k, g.ko, g.Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
+        g.k_sb, g.k_st, g.k_sh, _ = k.stride()
+    else:
+        g.Hk = 0
+    check(lib().dtt_rotary(C.byref(g), stream_ptr()), "dtt_rotary")
     return qo, ko
 
 
 class Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, freq, interleaved, amplitude):
-        qo, ko = _rotate(q, k, positions, freq, interleaved, amplitude, False)
+    def forward(ctx, q, k, positions, freq, g):
         ctx.save_for_backward(positions, freq)
-        ctx.cfg = (interleaved, amplitude)
+        ctx.call = g
         ctx.set_materialize_grads(False)
-        return qo, ko
+        return _rotate(q, k, _again(g))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
-        positions, freq = ctx.saved_tensors
-        have = [_rows(t) for t in (dq, dk) if t is not None]
-        got = _rotate(have[0], have[1] if len(have) > 1 else None, positions, freq, *ctx.cfg, True) if have else (None, None)
+        ctx.saved_tensors                                                     # (raises if positions or freq were overwritten)
+        g = _again(ctx.call)
+        g.back = 1
         if dq is None:
-            got = (None, got[0])
-        return got + (None, None, None, None)
+            return (None, None if dk is None else _rotate(_inner(dk), None, g)[0], None, None, None)
+        return _rotate(_inner(dq), None if dk is None else _inner(dk), g) + (None, None, None)
 
 
 def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
@@ -448,20 +442,39 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
     (rotary_frequencies).  Angles are formed in float64, so positions far into a stream keep their precision.  Returns the
     turned q and k (or q alone where k is None); differentiable in both."""
     name = "rotary"
-    _need(torch.is_tensor(q) and q.dim() == 4 and (k is None or (k.dim() == 4 and k.shape[:2] == q.shape[:2] and
-                                                                k.shape[3] == q.shape[3] and k.dtype == q.dtype)),
-          f"{name}: q and k must be [B, T, H, dh] of one dtype, with one B, T and dh")
-    _same(name, q, ("k", k), ("positions", positions), ("freq", freq))
-    dtype_code(q.dtype)
+    if not torch.is_tensor(q) or q.dim() != 4:
+        _fail(name, "q must be [B, T, H, dh]")
+    _on_gpu(name, q)
     B, T, _, dh = q.shape
-    _need(positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) in ((T,), (B, T)),
-          f"{name}: positions must be int32 or int64 [T] or [B, T], got {positions.dtype} {tuple(positions.shape)}")
-    _need(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous() and 0 < 2 * freq.shape[0] <= min(dh, 4096),
-          f"{name}: freq must be a contiguous float64 vector of 1 to dh / 2 elements")
+    dev = q.device
+    if k is not None:
+        ks = k.shape
+        if len(ks) != 4 or ks[0] != B or ks[1] != T or ks[3] != dh or k.dtype is not q.dtype:
+            _fail(name, f"q {tuple(q.shape)} {q.dtype} and k {tuple(ks)} {k.dtype} must agree in all but heads")
+        _beside(name, q, "k", k)
+    pd = positions.dim()
+    if positions.dtype not in (I64, I32) or positions.shape != ((T,) if pd == 1 else (B, T)):
+        _fail(name, f"positions must be int32 or int64 [T] or [B, T], got {positions.dtype} {tuple(positions.shape)}")
+    if freq.dtype is not F64 or freq.dim() != 1 or not freq.is_contiguous() or not 0 < 2 * freq.shape[0] <= min(dh, 4096):
+        _fail(name, "freq must be a contiguous float64 vector of 1 to dh / 2 elements (2048 at most)")
+    if positions.device != dev or freq.device != dev:
+        _fail(name, f"positions and freq must be on {dev}")
     if q.numel() == 0 or (k is not None and k.numel() == 0):
-        _need(q.numel() == 0 and (k is None or k.numel() == 0), f"{name}: q and k must both have heads")
+        if q.numel() or (k is not None and k.numel()):
+            _fail(name, "q and k must both have heads")
         return q.clone() if k is None else (q.clone(), k.clone())
-    q, k = _rows(q), _rows(k) if k is not None else None
-    args = (positions, freq, bool(interleaved), float(amplitude))
-    out = Rotary.apply(q, k, *args) if _wants_grad(q, k) else _rotate(q, k, *args, False)
-    return out[0] if k is None else out
+    if q.get_device() != _device():
+        with torch.cuda.device(dev):
+            return rotary(q, k, positions, freq, interleaved, amplitude)
+    g = DttRotary(B=B, T=T, dh=dh, r=2 * freq.shape[0], interleaved=1 if interleaved else 0, pos64=1 if positions.dtype is I64 else 0,
+                  dtype=1 if q.dtype is BF16 else 0, amplitude=amplitude)
+    g.positions, g.freq, g.p_st = positions.data_ptr(), freq.data_ptr(), positions.stride(-1)
+    if pd == 2:
+        g.p_sb = positions.stride(0)
+    q = _inner(q)
+    if k is None:
+        return Rotary.apply(q, None, positions, freq, g)[0] if torch.is_grad_enabled() and q.requires_grad else _rotate(q, None, g)[0]
+    k = _inner(k)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return Rotary.apply(q, k, positions, freq, g)
+    return _rotate(q, k, g)
