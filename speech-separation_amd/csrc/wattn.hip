@@ -135,6 +135,32 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32
         }
 }
 
+// Raw scores x of 32 keys -> weights 2^(sc x - m), with the running reference m and sum l of this lane's query.  The reference
+// need not be the maximum: it follows it only when a row's maximum has grown by more than 2^8 over it (weights up to 256
+// keep all their relative precision in fp32 and bf16), so that the accumulators are hardly ever rescaled.
+template <int DH>
+__device__ __forceinline__ void softmax_tile(f32x16_t& x, float& m, float& l, f32x16_t (&o)[DH / 32], float sc) {
+    float top = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+    if (__any(top > m + 8.f)) {
+        const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+        m = mn;
+#pragma unroll
+        for (int c = 0; c < DH / 32; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] *= al;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
+        l += x[r];
+    }
+}
+
 // The key tiles (of N keys) that the query rows at positions p0 .. p1 see: [0, a) holds first tokens only, [b, c] the window.
 struct Tiles { int a, b, c; };
 template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0, int p1, int klen) {
@@ -149,7 +175,7 @@ template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0
 }
 
 template <typename T, int DH>
-__global__ __launch_bounds__(NTH) void wattn_fwd_kernel(const WaP p) {
+__global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     __shared__ __align__(16) T ks[BN * I::LD];
@@ -210,26 +236,7 @@ __global__ __launch_bounds__(NTH) void wattn_fwd_kernel(const WaP p) {
                     x[r] = see ? x[r] : -INFINITY;
                 }
             }
-            float top = x[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
-            const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
-            const float al = __builtin_amdgcn_exp2f(m - mu);
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
-                sum += x[r];
-            }
-            l = fmaf(l, al, sum);
-            m = mn;
-            if (__any(al != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < DH / 32; ++c)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[c][r] *= al;
-            }
+            softmax_tile<DH>(x, m, l, o, sc);
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
 #pragma unroll
             for (int ct = 0; ct < DH / 32; ++ct)
@@ -251,7 +258,7 @@ __global__ __launch_bounds__(NTH) void wattn_fwd_kernel(const WaP p) {
 
 // dq, and D = sum(dO O) per row for the dk / dv launch behind it
 template <typename T, int DH>
-__global__ __launch_bounds__(NTH) void wattn_dq_kernel(const WaP p) {
+__global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     __shared__ __align__(16) T ks[BN * I::LD];
@@ -313,19 +320,24 @@ __global__ __launch_bounds__(NTH) void wattn_dq_kernel(const WaP p) {
         for (int s = 0; s < BN / 32; ++s) {
             const int js = j0 + 32 * s;
             if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
-            f32x16_t x = zero_acc(), y = zero_acc();
+            f32x16_t x = zero_acc(), y;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[r] = -dd;                      // y = dP - D
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
+            if (!full) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = js + acc_row(r, lh);
-                const bool see = full || (j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen);
-                const float e = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse));
-                x[r] = see ? e * (y[r] - dd) : 0.f;
+                for (int r = 0; r < 16; ++r) {
+                    const int j = js + acc_row(r, lh);
+                    const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
+                    x[r] = see ? x[r] : -INFINITY;
+                }
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * y[r];
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
 #pragma unroll
             for (int ct = 0; ct < DH / 32; ++ct)
@@ -347,7 +359,7 @@ __global__ __launch_bounds__(NTH) void wattn_dq_kernel(const WaP p) {
 // 32-row tile against the first tokens' rows; those and tile 0's own sums go to fp32 partials that
 // wattn_sink_sum_kernel adds in order.
 template <typename T, int DH>
-__global__ __launch_bounds__(NTH) void wattn_dkv_kernel(const WaP p, int main) {
+__global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn_dkv_kernel(const WaP p, int main) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     __shared__ __align__(16) T qs[QN * I::LD];
@@ -420,23 +432,33 @@ __global__ __launch_bounds__(NTH) void wattn_dkv_kernel(const WaP p, int main) {
             if (far && s != wave) continue;
             const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
-            f32x16_t x = zero_acc(), y = zero_acc();
+            f32x16_t x = zero_acc(), y;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const float4 ds = *reinterpret_cast<const float4*>(&st[1][32 * s + 8 * r4 + 4 * lh]);
+                y[4 * r4] = -ds.x, y[4 * r4 + 1] = -ds.y, y[4 * r4 + 2] = -ds.z, y[4 * r4 + 3] = -ds.w;     // y = dP - D
+            }
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), kf[c], x);
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
             const bool full = kw + 31 <= pr + p.right && (kw >= pr + 31 - p.left || kw + 31 < p.sinks) && kw + 31 < klen;
+            if (!full) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int pp = pr + acc_row(r, lh);
+                    const bool see = j <= pp + p.right && (j >= pp - p.left || j < p.sinks) && j < klen;
+                    x[r] = see ? x[r] : -INFINITY;
+                }
+            }
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const float4 ls = *reinterpret_cast<const float4*>(&st[0][32 * s + 8 * r4 + 4 * lh]);
-                const float4 ds = *reinterpret_cast<const float4*>(&st[1][32 * s + 8 * r4 + 4 * lh]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * r4 + e, pp = pr + 8 * r4 + 4 * lh + e;
-                    const bool see = full || (j <= pp + p.right && (j >= pp - p.left || j < p.sinks) && j < klen);
-                    const float pv = see ? __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(&ls.x)[e])) : 0.f;
-                    x[r] = pv;
-                    y[r] = see ? pv * (y[r] - (&ds.x)[e]) : 0.f;
+                    const int r = 4 * r4 + e;
+                    x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(&ls.x)[e]));
+                    y[r] *= x[r];
                 }
             }
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
@@ -449,6 +471,10 @@ __global__ __launch_bounds__(NTH) void wattn_dkv_kernel(const WaP p, int main) {
                     MM<T>::mma(tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct), df[c], dk[ct]);
                 }
         }
+    }
+    if (j >= klen) {                                                      // padding: what was read of it stays out
+#pragma unroll
+        for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
     }
     if (p.nchunk > 0 && j < p.sinks && (!far || wave < 2)) {              // first tokens: fp32 partials, summed in order behind
         const int at = far ? 1 + 2 * ch + wave : 0;
@@ -496,7 +522,7 @@ __device__ __forceinline__ int slot_of(int64_t pos, int S, int W) { return pos <
 // slots; a wave takes every fourth 32-slot tile of it.  K is read from memory in fragment order; V goes through
 // a wave's own LDS image for the transposing read.
 template <typename T, int DH>
-__global__ __launch_bounds__(NTH) void wattn_step_kernel(const WsP p) {
+__global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel(const WsP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     constexpr int NV = (32 * I::NP + 63) / 64;
@@ -560,26 +586,7 @@ __global__ __launch_bounds__(NTH) void wattn_step_kernel(const WsP p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = js + acc_row(r, lh) < valid ? x[r] : -INFINITY;
         }
-        float top = x[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
-        const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - mu);
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
-            sum += x[r];
-        }
-        l = fmaf(l, al, sum);
-        m = mn;
-        if (__any(al != 1.f)) {
-#pragma unroll
-            for (int c = 0; c < DH / 32; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[c][r] *= al;
-        }
+        softmax_tile<DH>(x, m, l, o, sc);
         const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the image's writes ahead of its reads (one wave)
 #pragma unroll
