@@ -17,8 +17,8 @@
 #include "../../include/dtt_hip.h"
 
 namespace {
-constexpr int NTH = 256, BM = 128, BN = 64;      // forward / dq: query rows of a workgroup (32 a wave), keys of a staged tile
-constexpr int KM = 128, QN = 64;                 // dk / dv: keys of a workgroup (32 a wave), query rows of a staged tile
+constexpr int NTH = 256, BN = 64;                // threads (dk / dv: up to twice that); keys of a staged tile (forward, dq)
+constexpr int QN = 64, MAX_SINKS = 128;          // dk / dv: query rows of a staged tile
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct WaP {
@@ -28,7 +28,7 @@ struct WaP {
     const int* len;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
     int B, Tq, Tk, Hq, Hk, G, left, right, sinks, offset;
-    int nt, nchunk, chunk, npart;                // tiles along the row axis; far-query chunks of the sinks' gradients
+    int nt, nchunk, chunk, npart, edge;          // tiles along the row axis; chunks of the rows from edge on (first tokens' gradients)
     float scale;
 };
 
@@ -96,21 +96,21 @@ __device__ __forceinline__ f32x16_t zero_acc() {
 __device__ __forceinline__ int acc_row(int r, int lh) { return (r & 3) + 8 * (r >> 2) + 4 * lh; }
 
 // R rows from `src` (row stride rs elements) into registers; rows outside [0, n) come from the zero page, never from memory
-template <typename T, int DH, int R> struct Stage {
-    static constexpr int NP = Img<T, DH>::NP, N = (R * NP + NTH - 1) / NTH;
+template <typename T, int DH, int R, int NT = NTH> struct Stage {
+    static constexpr int NP = Img<T, DH>::NP, N = (R * NP + NT - 1) / NT;
     Vec16<T> v[N];
     __device__ __forceinline__ void load(const T* src, int64_t rs, int r0, int n) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NTH, r = r0 + id / NP;
+            const int id = threadIdx.x + i * NT, r = r0 + id / NP;
             v[i] = ld16_pred<T>(src + (int64_t)r * rs + (id % NP) * Img<T, DH>::EPP, src, id < R * NP && r >= 0 && r < n);
         }
     }
     __device__ __forceinline__ void store(T* img) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NTH;
-            if (R * NP % NTH == 0 || id < R * NP) st16<T>(img + Img<T, DH>::at(id / NP, id % NP), v[i]);
+            const int id = threadIdx.x + i * NT;
+            if (R * NP % NT == 0 || id < R * NP) st16<T>(img + Img<T, DH>::at(id / NP, id % NP), v[i]);
         }
     }
 };
@@ -161,6 +161,20 @@ __device__ __forceinline__ void softmax_tile(f32x16_t& x, float& m, float& l, f3
     }
 }
 
+// A wave's accumulators to and from LDS, [register][lane]: waves that share rows add up their halves there
+template <int N> __device__ __forceinline__ void park(float* at, const f32x16_t (&a)[N], int lane) {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at[(c * 16 + r) * 64 + lane] = a[c][r];
+}
+template <int N> __device__ __forceinline__ void unpark(const float* at, f32x16_t (&a)[N], int lane, float mine, float theirs) {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) a[c][r] = fmaf(at[(c * 16 + r) * 64 + lane], theirs, a[c][r] * mine);
+}
+
 // The key tiles (of N keys) that the query rows at positions p0 .. p1 see: [0, a) holds first tokens only, [b, c] the window.
 struct Tiles { int a, b, c; };
 template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0, int p1, int klen) {
@@ -174,21 +188,26 @@ template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0
     return t;
 }
 
-template <typename T, int DH>
+// RG row groups of 32 a workgroup, each by SP waves that take its 32-key tiles in turn and join at the end
+template <typename T, int DH, int RG, int SP>
 __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
-    __shared__ __align__(16) T ks[BN * I::LD];
-    __shared__ __align__(16) T vs[BN * I::LD];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    constexpr int BM = 32 * RG;
+    __shared__ __align__(16) T img[2 * BN * I::LD];
+    __shared__ float ml[SP > 1 ? RG : 1][2][32];
+    T* ks = img;
+    T* vs = img + BN * I::LD;
+    static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
     int id = xcd_order(blockIdx.x, gridDim.x);
     const int g = id % p.G; id /= p.G;
     const int qt = id % p.nt; id /= p.nt;
     const int hk = id % p.Hk, b = id / p.Hk, h = hk * p.G + g;
     const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
-    const int i = qt * BM + wave * 32 + lr, pos = p.offset + i, pw = p.offset + qt * BM + wave * 32;
+    const int i = qt * BM + rg * 32 + lr, pos = p.offset + i, pw = p.offset + qt * BM + rg * 32;
     const T* q = (const T*)p.q + b * p.q_sb + (int64_t)min(i, p.Tq - 1) * p.q_st + h * p.q_sh;
-    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* kp = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
     Frag qf[DH / 16];
 #pragma unroll
@@ -205,7 +224,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
     if (count > 0) {
-        sk.load(k, p.k_st, t * BN, klen);
+        sk.load(kp, p.k_st, t * BN, klen);
         sv.load(v, p.v_st, t * BN, klen);
     }
     for (int n = 0; n < count; ++n) {
@@ -216,12 +235,12 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
         const int j0 = t * BN;
         t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
         if (n + 1 < count) {
-            sk.load(k, p.k_st, t * BN, klen);
+            sk.load(kp, p.k_st, t * BN, klen);
             sv.load(v, p.v_st, t * BN, klen);
         }
 #pragma unroll
-        for (int s = 0; s < BN / 32; ++s) {
-            const int js = j0 + 32 * s;
+        for (int k = 0; k < BN / 32 / SP; ++k) {
+            const int s = k * SP + sp, js = j0 + 32 * s;
             // nothing of this 32 x 32 tile is visible
             if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
             f32x16_t x = zero_acc();
@@ -245,6 +264,21 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
         }
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (SP > 1) {
+        float* at = reinterpret_cast<float*>(img) + rg * DH * 32;
+        __syncthreads();
+        if (sp) {
+            park(at, o, lane);
+            if (lh == 0) ml[rg][0][lr] = m, ml[rg][1][lr] = l;
+        }
+        __syncthreads();
+        if (sp) return;
+        const float m1 = ml[rg][0][lr], mn = fmaxf(m, m1), mu = mn == -INFINITY ? 0.f : mn;
+        const float a0 = __builtin_amdgcn_exp2f(m - mu), a1 = __builtin_amdgcn_exp2f(m1 - mu);
+        l = fmaf(ml[rg][1][lr], a1, l * a0);
+        m = mn;
+        unpark(at, o, lane, a0, a1);
+    }
     if (i >= p.Tq) return;
     const bool live = pos < qlen && l != 0.f;         // (l is at least 1 where anything is visible; NaN passes)
     T* out = (T*)p.out + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH;
@@ -257,24 +291,27 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
 }
 
 // dq, and D = sum(dO O) per row for the dk / dv launch behind it
-template <typename T, int DH>
+template <typename T, int DH, int RG, int SP>
 __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
-    __shared__ __align__(16) T ks[BN * I::LD];
-    __shared__ __align__(16) T vs[BN * I::LD];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    constexpr int BM = 32 * RG;
+    __shared__ __align__(16) T img[2 * BN * I::LD];
+    T* ks = img;
+    T* vs = img + BN * I::LD;
+    static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
     int id = xcd_order(blockIdx.x, gridDim.x);
     const int g = id % p.G; id /= p.G;
     const int qt = id % p.nt; id /= p.nt;
     const int hk = id % p.Hk, b = id / p.Hk, h = hk * p.G + g;
     const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
-    const int i = qt * BM + wave * 32 + lr, ic = min(i, p.Tq - 1), pos = p.offset + i, pw = p.offset + qt * BM + wave * 32;
+    const int i = qt * BM + rg * 32 + lr, ic = min(i, p.Tq - 1), pos = p.offset + i, pw = p.offset + qt * BM + rg * 32;
     const bool live = i < p.Tq && pos < qlen;
     const T* q = (const T*)p.q + b * p.q_sb + (int64_t)ic * p.q_st + h * p.q_sh;
     const T* go = (const T*)p.dout + b * p.g_sb + (int64_t)ic * p.g_st + h * p.g_sh;
     const T* oo = (const T*)p.o + ((int64_t)(b * p.Tq + ic) * p.Hq + h) * DH;
-    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* kp = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
     Frag qf[DH / 16], gf[DH / 16];
     float dd = 0.f;
@@ -291,7 +328,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
     dd += __shfl_xor(dd, 32, 64);
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
     const float lse = p.lse[at];
-    if (live && lh == 0) p.dd[at] = dd;
+    if (live && lh == 0 && sp == 0) p.dd[at] = dd;
     f32x16_t dq[DH / 32];
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
@@ -302,7 +339,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
     int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
     if (count > 0) {
-        sk.load(k, p.k_st, t * BN, klen);
+        sk.load(kp, p.k_st, t * BN, klen);
         sv.load(v, p.v_st, t * BN, klen);
     }
     for (int n = 0; n < count; ++n) {
@@ -313,12 +350,12 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
         const int j0 = t * BN;
         t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
         if (n + 1 < count) {
-            sk.load(k, p.k_st, t * BN, klen);
+            sk.load(kp, p.k_st, t * BN, klen);
             sv.load(v, p.v_st, t * BN, klen);
         }
 #pragma unroll
-        for (int s = 0; s < BN / 32; ++s) {
-            const int js = j0 + 32 * s;
+        for (int k = 0; k < BN / 32 / SP; ++k) {
+            const int s = k * SP + sp, js = j0 + 32 * s;
             if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
             f32x16_t x = zero_acc(), y;
 #pragma unroll
@@ -345,6 +382,14 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
                 for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct), pf[c], dq[ct]);
         }
     }
+    if constexpr (SP > 1) {
+        float* mem = reinterpret_cast<float*>(img) + rg * DH * 32;
+        __syncthreads();
+        if (sp) park(mem, dq, lane);
+        __syncthreads();
+        if (sp) return;
+        unpark(mem, dq, lane, 1.f, 1.f);
+    }
     if (i >= p.Tq) return;
     if (!live || lse == INFINITY) {
 #pragma unroll
@@ -353,19 +398,30 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
     store_rows<T, DH>((T*)p.dq + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH, dq, p.scale, lh);
 }
 
-// dk, dv: a workgroup owns KM keys of one key head (32 a wave) and walks the query rows that see them, over the heads of its
-// group: no atomics, one order of additions.  First tokens are seen by every later row: the rows beyond the window of
-// tile 0 are cut into chunks, each a workgroup of its own (blockIdx.x >= main) whose waves 0 and 1 take every other
-// 32-row tile against the first tokens' rows; those and tile 0's own sums go to fp32 partials that
-// wattn_sink_sum_kernel adds in order.
-template <typename T, int DH>
-__global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn_dkv_kernel(const WaP p, int main) {
+// dk, dv: a workgroup owns 32 KG keys of one key head (32 a wave) and walks the query rows that see them, over the heads of
+// its group: no atomics, one order of additions.  SP waves share the same keys and take the 32-row tiles in turn; their
+// sums meet in LDS at the end.  First tokens are seen by every later row: the rows from p.edge on are left out of the
+// walk of the key tiles that hold them and cut into chunks, each a workgroup of its own (blockIdx.x >= main) whose waves 0
+// and 1 take every other 32-row tile against the first tokens' rows; those and the key tiles' own sums go to fp32 partials
+// that wattn_sink_sum_kernel adds in order.
+template <typename T, int DH, int KG, int SP>
+__global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * SP == 8) ? 2 : 1) void wattn_dkv_kernel(const WaP p, int main) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
-    __shared__ __align__(16) T qs[QN * I::LD];
-    __shared__ __align__(16) T gs[QN * I::LD];
+    // V's fragments (and K's) are read from LDS where with both sums, both tiles and the next rows on their way they would
+    // exceed the registers of two waves a SIMD (fp32: of one)
+    constexpr int KM = 32 * KG, NT = KG * SP * 64;
+    constexpr bool VL = DH >= 96, KL = DH == 128 && sizeof(T) == 2 && KG * SP == 8;
+    constexpr int TILE = QN * I::LD, OWN = KM * I::LD, N = 2 * TILE + (VL ? OWN : 0) + (KL ? OWN : 0);
+    constexpr int PARK = SP > 1 ? KG * DH * 128 / (int)sizeof(T) : 0;
+    static_assert(SP <= QN / 32, "a 32-row tile of a staged one for every wave that shares keys");
+    __shared__ __align__(16) T mem[N > PARK ? N : PARK];
     __shared__ __align__(16) float st[2][QN];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    T* qs = mem;
+    T* gs = mem + TILE;
+    T* vimg = mem + 2 * TILE;
+    T* kimg = vimg + OWN;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, kg = SP > 1 ? wave % KG : wave, sp = SP > 1 ? wave / KG : 0;
     const bool far = (int)blockIdx.x >= main;
     int id = far ? blockIdx.x - main : xcd_order(blockIdx.x, main);
     const int ns32 = (p.sinks + 31) / 32;
@@ -375,35 +431,43 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn
         kw = id % ns32 * 32; id /= ns32;
     } else {
         kt = id % p.nt; id /= p.nt;
-        kw = kt * KM + wave * 32;
+        kw = kt * KM + kg * 32;
     }
     const int hk = id % p.Hk, b = id / p.Hk;
     const int qlen = p.len ? p.len[b] : INT_MAX, klen = min(p.Tk, qlen);
     const int qrows = min(p.Tq, qlen < INT_MAX ? max(0, qlen - p.offset) : p.Tq);       // live query rows
     // query rows of this workgroup: [r0, r1)
-    const int edge = min(p.Tq, max(0, KM + p.left - p.offset));          // first row beyond the window of tile 0
     int r0, r1;
     if (far) {
-        r0 = edge + ch * p.chunk;
+        r0 = p.edge + ch * p.chunk;
         r1 = min(r0 + p.chunk, qrows);
     } else {
         r0 = max(0, kt * KM - p.right - p.offset);
         r1 = min(qrows, max(0, kt * KM + KM + p.left - p.offset));
+        if (kt * KM < p.sinks) r1 = min(qrows, p.edge);                  // (and no chunks: all rows)
     }
     const int j = kw + lr, jc = min(j, p.Tk - 1);
-    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh + (int64_t)jc * p.k_st;
-    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh + (int64_t)jc * p.v_st;
-    Frag kf[DH / 16], vf[DH / 16];
+    const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    Frag kf[KL ? 1 : DH / 16], vf[VL ? 1 : DH / 16];
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c) {
-        kf[c] = MM<T>::ldfrag(k + 16 * c + 8 * lh);
-        vf[c] = MM<T>::ldfrag(v + 16 * c + 8 * lh);
+        if constexpr (!KL) kf[c] = MM<T>::ldfrag(k + (int64_t)jc * p.k_st + 16 * c + 8 * lh);
+        if constexpr (!VL) vf[c] = MM<T>::ldfrag(v + (int64_t)jc * p.v_st + 16 * c + 8 * lh);
     }
+    if constexpr (VL) {                           // (rows behind the keys: zeros; seen by the barrier ahead of the first tile)
+        for (int e = threadIdx.x; e < KM * I::NP; e += NT) {
+            const int r = e / I::NP, pc = e % I::NP, jv = (far ? kw : kt * KM) + r;
+            st16<T>(vimg + I::at(r, pc), ld16_pred<T>(v + (int64_t)jv * p.v_st + pc * I::EPP, v, jv < klen));
+            if constexpr (KL) st16<T>(kimg + I::at(r, pc), ld16_pred<T>(k + (int64_t)jv * p.k_st + pc * I::EPP, k, jv < klen));
+        }
+    }
+    const int vr = (far ? 0 : kg * 32) + lr;      // this lane's row there
     f32x16_t dk[DH / 32], dv[DH / 32];
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
     const float sc = p.scale * LOG2E;
-    Stage<T, DH, QN> sq, sg;
+    Stage<T, DH, QN, NT> sq, sg;
     const int per = r1 > r0 ? (r1 - r0 + QN - 1) / QN : 0, count = per * p.G;
     float sl = 0.f, sd = 0.f;
     auto load = [&](int n) {
@@ -428,8 +492,9 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn
         const int i0 = r0 + n % per * QN;
         if (n + 1 < count) load(n + 1);
 #pragma unroll
-        for (int s = 0; s < QN / 32; ++s) {
-            if (far && s != wave) continue;
+        for (int it = 0; it < (SP > 1 ? 1 : QN / 32); ++it) {
+            const int s = far ? wave : SP > 1 ? sp : it;                  // far: waves 0 and 1, one tile each
+            if (far && (it || wave >= QN / 32)) continue;
             const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
             f32x16_t x = zero_acc(), y;
@@ -439,9 +504,15 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn
                 y[4 * r4] = -ds.x, y[4 * r4 + 1] = -ds.y, y[4 * r4 + 2] = -ds.z, y[4 * r4 + 3] = -ds.w;     // y = dP - D
             }
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), kf[c], x);
+            for (int c = 0; c < DH / 16; ++c) {
+                if constexpr (KL) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), nat_frag<T, DH>(kimg, vr, c, lh), x);
+                else MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), kf[c], x);
+            }
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
+            for (int c = 0; c < DH / 16; ++c) {
+                if constexpr (VL) MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), nat_frag<T, DH>(vimg, vr, c, lh), y);
+                else MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
+            }
             const bool full = kw + 31 <= pr + p.right && (kw >= pr + 31 - p.left || kw + 31 < p.sinks) && kw + 31 < klen;
             if (!full) {
 #pragma unroll
@@ -472,11 +543,22 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn
                 }
         }
     }
+    if (SP > 1 && !far) {
+        float* at = reinterpret_cast<float*>(mem) + kg * DH * 32;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            __syncthreads();
+            if (sp) park(at, w ? dv : dk, lane);
+            __syncthreads();
+            if (!sp) unpark(at, w ? dv : dk, lane, 1.f, 1.f);
+        }
+        if (sp) return;
+    }
     if (j >= klen) {                                                      // padding: what was read of it stays out
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
     }
-    if (p.nchunk > 0 && j < p.sinks && (!far || wave < 2)) {              // first tokens: fp32 partials, summed in order behind
+    if (p.nchunk > 0 && j < p.sinks && (!far || wave < QN / 32)) {              // first tokens: fp32 partials, summed in order behind
         const int at = far ? 1 + 2 * ch + wave : 0;
         float* d = p.part + ((((int64_t)b * p.Hk + hk) * p.npart + at) * p.sinks + j) * 2 * DH;
         store_rows<float, DH>(d, dk, p.scale, lh);
@@ -488,19 +570,24 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && DH <= 64 ? 2 : 1) void wattn
     store_rows<T, DH>((T*)p.dv + row, dv, 1.f, lh);
 }
 
-// first tokens' dk, dv: the partials in their order
+// first tokens' dk, dv: the partials in one order (four slices of them side by side, then the four sums)
 template <typename T>
 __global__ __launch_bounds__(NTH) void wattn_sink_sum_kernel(const WaP p, int dh, int64_t n) {
-    const int64_t id = (int64_t)blockIdx.x * NTH + threadIdx.x;
-    if (id >= n) return;
-    const int d = (int)(id % (2 * dh));
-    const int64_t bj = id / (2 * dh);
-    const int j = (int)(bj % p.sinks);
-    const int64_t bh = bj / p.sinks;
+    __shared__ float part[4][64];
+    const int e = threadIdx.x & 63, sl = threadIdx.x >> 6;
+    const int64_t id = (int64_t)blockIdx.x * 64 + e;
+    const int64_t c = id < n ? id : n - 1;
+    const int d = (int)(c % (2 * dh));
+    const int64_t bj = c / (2 * dh), bh = bj / p.sinks, step = (int64_t)p.sinks * 2 * dh;
+    const int j = (int)(bj % p.sinks), per = (p.npart + 3) / 4, k1 = min(p.npart, (sl + 1) * per);
     const float* s = p.part + (bh * p.npart * p.sinks + j) * 2 * dh + d;
     float sum = 0.f;
-    for (int k = 0; k < p.npart; ++k) sum += s[(int64_t)k * p.sinks * 2 * dh];
-    if (j >= p.Tk) return;
+#pragma unroll 8
+    for (int k = sl * per; k < k1; ++k) sum += s[k * step];
+    part[sl][e] = sum;
+    __syncthreads();
+    if (sl || id >= n) return;
+    sum = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
     const int64_t row = ((bh / p.Hk * p.Tk + j) * p.Hk + bh % p.Hk) * dh;
     if (d < dh) stf((T*)p.dk + row + d, sum);
     else stf((T*)p.dv + row + d - dh, sum);
@@ -688,7 +775,7 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     DTT_CHECK(g->DH == 32 || g->DH == 64 || g->DH == 96 || g->DH == 128, "%s: head width %d (32, 64, 96 or 128)", what, g->DH);
     DTT_CHECK(g->left >= 0 && g->right >= 0 && g->offset >= 0 && g->left < (1 << 29) && g->right < (1 << 29) && g->offset < (1 << 29) &&
               g->Tq < (1 << 29) && g->Tk < (1 << 29), "%s: window, offset and lengths must be in [0, 2^29)", what);
-    DTT_CHECK(g->sinks >= 0 && g->sinks <= KM, "%s: sinks=%d (0 to %d)", what, g->sinks, KM);
+    DTT_CHECK(g->sinks >= 0 && g->sinks <= MAX_SINKS, "%s: sinks=%d (0 to %d)", what, g->sinks, MAX_SINKS);
     DTT_CHECK(g->scale > 0.f && g->scale < INFINITY, "%s: scale=%g must be positive", what, g->scale);
     DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
     p = WaP{};
@@ -707,15 +794,20 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     return 0;
 }
 
-// chunks of the rows beyond tile 0's window that see the first tokens
+// The rows that see first tokens from beyond the windows of their key tiles, and the chunks they are cut into.  Short ones
+// keep the chunks' workgroups below the time of a key tile's.
 void far_chunks(WaP& p) {
-    const int64_t edge = (int64_t)KM + p.left - p.offset, far = p.Tq - (edge > 0 ? edge : 0);
-    p.nchunk = 0;
-    p.chunk = 512;
-    if (p.sinks > 0 && far > 0) p.nchunk = (int)((far + p.chunk - 1) / p.chunk);
+    const int64_t edge = (int64_t)MAX_SINKS + p.left - p.offset;          // behind the window of every tile with first tokens
+    p.edge = p.sinks == 0 || edge >= p.Tq ? p.Tq : edge > 0 ? (int)edge : 0;
+    p.chunk = 128;
+    p.nchunk = p.sinks ? (p.Tq - p.edge + p.chunk - 1) / p.chunk : 0;
     p.npart = 1 + 2 * p.nchunk;
 }
 int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk * p.npart * p.sinks * 2 * dh * 4 : 0; }
+
+// Few rows: half of them a workgroup, two waves on each (the walk over its keys half as long).  512 workgroups are two a CU.
+bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
+bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
 
 #define WA_DH(FN, T)                                                              \
     do {                                                                          \
@@ -732,11 +824,17 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_fwd")) return rc;
     DTT_CHECK(g->out && aligned16(g->out), "dtt_wattn_fwd: null or unaligned output");
-    p.nt = (p.Tq + BM - 1) / BM;
+    const bool split = split_rows(p);
+    const int bm = split ? 64 : 128;
+    p.nt = (p.Tq + bm - 1) / bm;
     const int64_t grid = (int64_t)p.B * p.Hq * p.nt;
     DTT_CHECK(grid < (1ll << 31), "dtt_wattn_fwd: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define FWD(T, D) hipLaunchKernelGGL((wattn_fwd_kernel<T, D>), dim3((unsigned)grid), dim3(NTH), 0, s, p)
+#define FWD(T, D)                                                                                                      \
+    do {                                                                                                               \
+        if (split) hipLaunchKernelGGL((wattn_fwd_kernel<T, D, 2, 2>), dim3((unsigned)grid), dim3(NTH), 0, s, p);       \
+        else hipLaunchKernelGGL((wattn_fwd_kernel<T, D, 4, 1>), dim3((unsigned)grid), dim3(NTH), 0, s, p);             \
+    } while (0)
     WA_DISPATCH(FWD);
 #undef FWD
     DTT_LAUNCH_CHECK();
@@ -762,19 +860,25 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     DTT_CHECK(need == 0 || (g->ws && aligned16(g->ws) && g->ws_bytes >= need), "dtt_wattn_bwd: workspace of %lld bytes, %lld given",
               (long long)need, (long long)g->ws_bytes);
     p.part = (float*)g->ws;
-    p.nt = (p.Tq + BM - 1) / BM;
+    const bool split = split_rows(p), splitk = split_keys(p);
+    const int bm = split ? 64 : 128, km = splitk ? 64 : 128;
+    p.nt = (p.Tq + bm - 1) / bm;
     WaP pk = p;
-    pk.nt = (p.Tk + KM - 1) / KM;
+    pk.nt = (p.Tk + km - 1) / km;
     const int64_t gq = (int64_t)p.B * p.Hq * p.nt, gk = (int64_t)p.B * p.Hk * pk.nt;
     const int64_t gf = (int64_t)p.B * p.Hk * p.nchunk * ((p.sinks + 31) / 32), n = (int64_t)p.B * p.Hk * p.sinks * 2 * g->DH;
     DTT_CHECK(gq < (1ll << 31) && gk + gf < (1ll << 31), "dtt_wattn_bwd: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define BWD(T, D)                                                                                                    \
-    do {                                                                                                             \
-        hipLaunchKernelGGL((wattn_dq_kernel<T, D>), dim3((unsigned)gq), dim3(NTH), 0, s, p);                         \
-        hipLaunchKernelGGL((wattn_dkv_kernel<T, D>), dim3((unsigned)(gk + gf)), dim3(NTH), 0, s, pk, (int)gk);       \
-        if (p.nchunk)                                                                                                \
-            hipLaunchKernelGGL((wattn_sink_sum_kernel<T>), dim3((unsigned)((n + NTH - 1) / NTH)), dim3(NTH), 0, s, p, g->DH, n); \
+    const dim3 dq((unsigned)gq), dkv((unsigned)(gk + gf));
+#define BWD(T, D)                                                                                                                  \
+    do {                                                                                                                           \
+        constexpr int SP = sizeof(T) == 2 ? 2 : 1;                                                                                 \
+        if (split) hipLaunchKernelGGL((wattn_dq_kernel<T, D, 2, 2>), dq, dim3(NTH), 0, s, p);                                      \
+        else hipLaunchKernelGGL((wattn_dq_kernel<T, D, 4, 1>), dq, dim3(NTH), 0, s, p);                                            \
+        if (splitk) hipLaunchKernelGGL((wattn_dkv_kernel<T, D, 2, 2>), dkv, dim3(NTH), 0, s, pk, (int)gk);                         \
+        else hipLaunchKernelGGL((wattn_dkv_kernel<T, D, 4, SP>), dkv, dim3(NTH * SP), 0, s, pk, (int)gk);                          \
+        if (p.nchunk)                                                                                                              \
+            hipLaunchKernelGGL((wattn_sink_sum_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(NTH), 0, s, p, g->DH, n);   \
     } while (0)
     WA_DISPATCH(BWD);
 #undef BWD
