@@ -488,7 +488,7 @@ int dtt_rotary(const DttRotary* g, void* stream);
 /* Windowed attention with first tokens that stay visible: the query at position p = offset + i sees key j where
  * j <= p + right and (j >= p - left or j < sinks); softmax(scale * q k^T) v over those; a row that sees none is zero.
  * lengths [B] (NULL: none): positions from lengths[b] on are padding: keys there are never read, rows there are zero and
- * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides, every row on 16 bytes; out, dq
+ * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides (rows of one head DH to 2^22 elements apart, every row on 16 bytes); out, dq
  * [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
  * lse [B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call; dd: the same size, scratch of
  * the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give equal bits. */

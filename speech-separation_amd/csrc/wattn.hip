@@ -95,23 +95,38 @@ __device__ __forceinline__ f32x16_t zero_acc() {
 }
 __device__ __forceinline__ int acc_row(int r, int lh) { return (r & 3) + 8 * (r >> 2) + 4 * lh; }
 
-// R rows from `src` (row stride rs elements) into registers; rows outside [0, n) come from the zero page, never from memory
+// R rows (row stride rs elements) into registers and on into an LDS image.  The tile's rows are a buffer of their own whose
+// size ends with the last valid row, so that rows behind it read as zeros without a predicate, and a lane's offsets are
+// the same 32-bit numbers for every tile (address arithmetic per lane was a quarter of
+// the forward kernel's vector instructions).  Needs DH <= rs <= 2^22 (checked on the host).
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 template <typename T, int DH, int R, int NT = NTH> struct Stage {
-    static constexpr int NP = Img<T, DH>::NP, N = (R * NP + NT - 1) / NT;
-    Vec16<T> v[N];
+    typedef Img<T, DH> I;
+    static constexpr int N = (R * I::RP + NT - 1) / NT;
+    u32x4_t v[N];
+    static constexpr int ROWS = NT / I::RP;       // rows between a lane's pieces
+    uint32_t off, step;
+    int at[2];
+    __device__ __forceinline__ explicit Stage(int64_t rs) {
+        const int r = threadIdx.x / I::RP, pc = threadIdx.x % I::RP;
+        // (a lane without a piece of its own: beyond every buffer)
+        off = pc < I::NP && r < R ? (uint32_t)(r * (int)rs + pc * I::EPP) * sizeof(T) : 0x80000000u;
+        step = (uint32_t)(ROWS * (int)rs) * sizeof(T);
+        at[0] = I::at(r, pc);                     // (the swizzle repeats every 16 rows: one place, or two in turn)
+        at[1] = I::at(r + ROWS, pc) - ROWS * I::LD;
+        static_assert(N == 1 || ROWS % 8 == 0, "");
+    }
     __device__ __forceinline__ void load(const T* src, int64_t rs, int r0, int n) {
+        const int rows = min(n - r0, R);
+        const int bytes = rows > 0 ? ((rows - 1) * (int)rs + DH) * (int)sizeof(T) : 0;
+        const __amdgpu_buffer_rsrc_t b = __builtin_amdgcn_make_buffer_rsrc((void*)(src + (int64_t)r0 * rs), 0, bytes, 0x00027000);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NT, r = r0 + id / NP;
-            v[i] = ld16_pred<T>(src + (int64_t)r * rs + (id % NP) * Img<T, DH>::EPP, src, id < R * NP && r >= 0 && r < n);
-        }
+        for (int i = 0; i < N; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(b, off + i * step, 0, 0);
     }
     __device__ __forceinline__ void store(T* img) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int id = threadIdx.x + i * NT;
-            if (R * NP % NT == 0 || id < R * NP) st16<T>(img + Img<T, DH>::at(id / NP, id % NP), v[i]);
-        }
+        for (int i = 0; i < N; ++i)
+            if (R * I::RP % NT == 0 || threadIdx.x < R * I::RP) *reinterpret_cast<u32x4_t*>(img + at[ROWS % 16 ? i & 1 : 0] + i * ROWS * I::LD) = v[i];
     }
 };
 
@@ -135,14 +150,16 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32
         }
 }
 
-// Raw scores x of 32 keys -> weights 2^(sc x - m), with the running reference m and sum l of this lane's query.  The reference
-// need not be the maximum: it follows it only when a row's maximum has grown by more than 2^8 over it (weights up to 256
-// keep all their relative precision in fp32 and bf16), so that the accumulators are hardly ever rescaled.
-template <int DH>
-__device__ __forceinline__ void softmax_tile(f32x16_t& x, float& m, float& l, f32x16_t (&o)[DH / 32], float sc) {
-    float top = x[0];
+// Raw scores x of 32 NX keys -> weights 2^(sc x - m), with the running reference m and sum l of this lane's query.  The
+// reference need not be the maximum: it follows it only when a row's maximum has grown by more than 2^8 over it (weights up
+// to 256 keep all their relative precision in fp32 and bf16), so that the accumulators are hardly ever rescaled.
+template <int DH, int NX>
+__device__ __forceinline__ void softmax_tile(f32x16_t (&x)[NX], float& m, float& l, f32x16_t (&o)[DH / 32], float sc) {
+    float top = x[0][0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+    for (int n = 0; n < NX; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
     if (__any(top > m + 8.f)) {
         const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -154,11 +171,15 @@ __device__ __forceinline__ void softmax_tile(f32x16_t& x, float& m, float& l, f3
             for (int r = 0; r < 16; ++r) o[c][r] *= al;
     }
     const float mu = m == -INFINITY ? 0.f : m;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -mu));
-        l += x[r];
-    }
+    for (int n = 0; n < NX; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[n][r] = __builtin_amdgcn_exp2f(fmaf(x[n][r], sc, -mu));
+            sum[r & 3] += x[n][r];
+        }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // A wave's accumulators to and from LDS, [register][lane]: waves that share rows add up their halves there
@@ -193,7 +214,7 @@ template <typename T, int DH, int RG, int SP>
 __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
-    constexpr int BM = 32 * RG;
+    constexpr int BM = 32 * RG, NX = 1;
     __shared__ __align__(16) T img[2 * BN * I::LD];
     __shared__ float ml[SP > 1 ? RG : 1][2][32];
     T* ks = img;
@@ -220,7 +241,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
 
     const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
     const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
-    Stage<T, DH, BN> sk, sv;
+    Stage<T, DH, BN> sk(p.k_st), sv(p.v_st);
     int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
     if (count > 0) {
@@ -240,27 +261,35 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
         }
 #pragma unroll
         for (int k = 0; k < BN / 32 / SP; ++k) {
-            const int s = k * SP + sp, js = j0 + 32 * s;
+            const int sub = k * SP + sp, ja = j0 + 32 * sub, jb = ja + 31;
             // nothing of this 32 x 32 tile is visible
-            if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
-            f32x16_t x = zero_acc();
+            if (ja > pw + 31 + p.right || (jb < pw - p.left && ja >= p.sinks) || ja >= klen) continue;
+            f32x16_t x[NX];
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
-            const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
-            if (!full) {
+            for (int n = 0; n < NX; ++n) x[n] = zero_acc();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = js + acc_row(r, lh);
-                    const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
-                    x[r] = see ? x[r] : -INFINITY;
-                }
+            for (int c = 0; c < DH / 16; ++c)
+#pragma unroll
+                for (int n = 0; n < NX; ++n) MM<T>::mma(nat_frag<T, DH>(ks, 32 * (sub + n) + lr, c, lh), qf[c], x[n]);
+            if (!(jb <= pw + p.right && (ja >= pw + 31 - p.left || jb < p.sinks) && jb < klen)) {
+#pragma unroll
+                for (int n = 0; n < NX; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = ja + 32 * n + acc_row(r, lh);
+                        const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
+                        x[n][r] = see ? x[n][r] : -INFINITY;
+                    }
             }
-            softmax_tile<DH>(x, m, l, o, sc);
-            const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+            softmax_tile<DH, NX>(x, m, l, o, sc);
 #pragma unroll
-            for (int ct = 0; ct < DH / 32; ++ct)
+            for (int n = 0; n < NX; ++n)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(vs, 32 * s + 16 * c, 32 * ct), pf[c], o[ct]);
+                for (int c = 0; c < 2; ++c) {
+                    const Frag pf = acc_frag<T>(x[n], c);
+#pragma unroll
+                    for (int ct = 0; ct < DH / 32; ++ct) MM<T>::mma(tr_frag_of<T, DH>(vs, 32 * (sub + n) + 16 * c, 32 * ct), pf, o[ct]);
+                }
         }
     }
     l += __shfl_xor(l, 32, 64);
@@ -292,10 +321,10 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
 
 // dq, and D = sum(dO O) per row for the dk / dv launch behind it
 template <typename T, int DH, int RG, int SP>
-__global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(const WaP p) {
+__global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_dq_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
-    constexpr int BM = 32 * RG;
+    constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
     __shared__ __align__(16) T img[2 * BN * I::LD];
     T* ks = img;
     T* vs = img + BN * I::LD;
@@ -335,7 +364,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
     const float sc = p.scale * LOG2E;
     const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
     const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
-    Stage<T, DH, BN> sk, sv;
+    Stage<T, DH, BN> sk(p.k_st), sv(p.v_st);
     int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
     if (count > 0) {
@@ -361,9 +390,10 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
 #pragma unroll
             for (int r = 0; r < 16; ++r) y[r] = -dd;                      // y = dP - D
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
-#pragma unroll
-            for (int c = 0; c < DH / 16; ++c) MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
+            for (int c = 0; c < DH / 16; ++c) {
+                MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
+                MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
+            }
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
             if (!full) {
 #pragma unroll
@@ -377,9 +407,9 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_dq_kernel(c
             for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * y[r];
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
 #pragma unroll
-            for (int ct = 0; ct < DH / 32; ++ct)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct), pf[c], dq[ct]);
+                for (int ct = 0; ct < DH / 32; ++ct) MM<T>::mma(tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct), pf[c], dq[ct]);
         }
     }
     if constexpr (SP > 1) {
@@ -467,7 +497,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
     const float sc = p.scale * LOG2E;
-    Stage<T, DH, QN, NT> sq, sg;
+    Stage<T, DH, QN, NT> sq(p.q_st), sg(p.g_st);
     const int per = r1 > r0 ? (r1 - r0 + QN - 1) / QN : 0, count = per * p.G;
     float sl = 0.f, sd = 0.f;
     auto load = [&](int n) {
@@ -659,7 +689,8 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
     int js = s0 + wave * 32;
     if (js < s1) load(js);
     for (; js < s1; js += 128) {
-        f32x16_t x = zero_acc();
+        f32x16_t xs[1] = {zero_acc()};
+        f32x16_t& x = xs[0];
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) MM<T>::mma(kf[c], qf[c], x);
         T* img = vs[wave];
@@ -673,7 +704,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = js + acc_row(r, lh) < valid ? x[r] : -INFINITY;
         }
-        softmax_tile<DH>(x, m, l, o, sc);
+        softmax_tile<DH, 1>(xs, m, l, o, sc);
         const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the image's writes ahead of its reads (one wave)
 #pragma unroll
@@ -783,10 +814,12 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
     // (strides of axes of one element do not count)
     const bool b = g->B > 1, tq = g->Tq > 1, tk = g->Tk > 1, hq = g->Hq > 1, hk = g->Hk > 1;
-    p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : 0; p.q_sh = hq ? g->q_sh : 0;
-    p.k_sb = b ? g->k_sb : 0; p.k_st = tk ? g->k_st : 0; p.k_sh = hk ? g->k_sh : 0;
-    p.v_sb = b ? g->v_sb : 0; p.v_st = tk ? g->v_st : 0; p.v_sh = hk ? g->v_sh : 0;
-    p.g_sb = b ? g->g_sb : 0; p.g_st = tq ? g->g_st : 0; p.g_sh = hq ? g->g_sh : 0;
+    p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : g->DH; p.q_sh = hq ? g->q_sh : 0;
+    p.k_sb = b ? g->k_sb : 0; p.k_st = tk ? g->k_st : g->DH; p.k_sh = hk ? g->k_sh : 0;
+    p.v_sb = b ? g->v_sb : 0; p.v_st = tk ? g->v_st : g->DH; p.v_sh = hk ? g->v_sh : 0;
+    p.g_sb = b ? g->g_sb : 0; p.g_st = tq && g->dout ? g->g_st : g->DH; p.g_sh = hq ? g->g_sh : 0;
+    const auto row_ok = [&](int64_t st) { return st >= g->DH && st <= (1 << 22); };
+    DTT_CHECK(row_ok(p.q_st) && row_ok(p.k_st) && row_ok(p.v_st) && row_ok(p.g_st), "%s: row strides must be DH to 2^22 elements", what);
     DTT_CHECK((p.q_sb | p.q_st | p.q_sh | p.k_sb | p.k_st | p.k_sh | p.v_sb | p.v_st | p.v_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->q) &&
               aligned16(g->k) && aligned16(g->v), "%s: rows must start on 16 bytes", what);
     p.B = g->B; p.Tq = g->Tq; p.Tk = g->Tk; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk;

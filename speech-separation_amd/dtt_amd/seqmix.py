@@ -63,6 +63,11 @@ def _rows16(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _rows_attn(t):
+    """What the whole-sequence attention reads: _rows16 with the rows of a head 1 row to 2^22 elements apart."""
+    return _rows16(t) if t.shape[-1] <= t.stride(1) <= 1 << 22 or t.shape[1] == 1 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _lengths(name, lengths, batch, first):
     if lengths is None:
         return None
@@ -242,7 +247,7 @@ class WindowAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do):
         q, k, v, lengths, out, lse = ctx.saved_tensors
-        do, g = _rows16(do), _again(ctx.call)
+        do, g = _rows_attn(do), _again(ctx.call)
         dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse)
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
         g.g_sb, g.g_st, g.g_sh, _ = do.stride()
@@ -299,7 +304,7 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
         with torch.cuda.device(q.device):
             return window_attention(q, k, v, left, right, sinks, lengths, offset, scale)
     cfg = (min(left, _BIG), min(right, _BIG), sinks, offset, q.shape[-1] ** -0.5 if scale is None else float(scale))
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    q, k, v = _rows_attn(q), _rows_attn(k), _rows_attn(v)
     return WindowAttention.apply(q, k, v, lengths, cfg) if grad else _attn_forward(q, k, v, lengths, cfg, False)[0]
 
 

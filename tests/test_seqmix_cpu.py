@@ -70,14 +70,15 @@ def test_attention_refusals():
 
     for kw, part in ((dict(B=0), "sizes"), (dict(Tq=0), "sizes"), (dict(Tk=0), "sizes"), (dict(Hq=3, Hk=2), "sizes"), (dict(DH=48), "head width"),
                      (dict(left=-1), "window"), (dict(right=-1), "window"), (dict(offset=-1), "window"), (dict(sinks=129), "sinks"),
-                     (dict(sinks=-1), "sinks"), (dict(q=None), "null"), (dict(q_st=33), "16 bytes"), (dict(k=BUF + 4), "16 bytes"),
+                     (dict(sinks=-1), "sinks"), (dict(q=None), "null"), (dict(q_st=33), "16 bytes"), (dict(q_st=24), "row strides"),
+                     (dict(k_st=(1 << 22) + 8), "row strides"), (dict(v_st=0), "row strides"), (dict(k=BUF + 4), "16 bytes"),
                      (dict(dtype=7), "dtype"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
                      (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale")):
         _fails(L.dtt_wattn_fwd(C.byref(g(**kw)), None), part)
         _fails(L.dtt_wattn_bwd(C.byref(g(**kw)), None), part)
     _fails(L.dtt_wattn_fwd(C.byref(g(out=None)), None), "output")
     _fails(L.dtt_wattn_bwd(C.byref(g(lse=None)), None), "null")
-    _fails(L.dtt_wattn_bwd(C.byref(g(g_st=2)), None), "16 bytes")
+    _fails(L.dtt_wattn_bwd(C.byref(g(g_st=33)), None), "16 bytes")
     far = dict(Tq=5000, Tk=5000, sinks=2)
     need = L.dtt_wattn_bwd_ws_bytes(C.byref(g(**far)))
     assert need > 0 and L.dtt_wattn_bwd_ws_bytes(C.byref(g())) == 0 and L.dtt_wattn_bwd_ws_bytes(None) == 0
