@@ -13,18 +13,24 @@
 #include "../../include/dtt_hip.h"
 
 namespace {
-constexpr int NTH = 256, TC = 4;                 // threads of a workgroup, steps a thread folds per tile
+constexpr int NTH = 256, TC = 8;                 // threads of a workgroup, steps a thread folds per tile
+constexpr int TSPLIT = 8;                        // time lanes of the split form
 
 template <typename T, int VEC> struct Raw;       // VEC consecutive channels as loaded
 template <> struct Raw<float, 4> {
     float4 v;
     __device__ __forceinline__ float get(int i) const { return (&v.x)[i]; }
-    __device__ __forceinline__ void set(int i, float f) { (&v.x)[i] = f; }
+    __device__ __forceinline__ void put(const float (&f)[4]) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <> struct Raw<float, 2> {
+    float2 v;
+    __device__ __forceinline__ float get(int i) const { return (&v.x)[i]; }
+    __device__ __forceinline__ void put(const float (&f)[2]) { v = make_float2(f[0], f[1]); }
 };
 template <> struct Raw<float, 1> {
     float v;
     __device__ __forceinline__ float get(int) const { return v; }
-    __device__ __forceinline__ void set(int, float f) { v = f; }
+    __device__ __forceinline__ void put(const float (&f)[1]) { v = f[0]; }
 };
 template <> struct Raw<bf16, 4> {
     uint2 v;
@@ -32,16 +38,17 @@ template <> struct Raw<bf16, 4> {
         const uint32_t w = (&v.x)[i >> 1];
         return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
     }
-    __device__ __forceinline__ void set(int i, float f) {
-        uint32_t& w = (&v.x)[i >> 1];
-        const uint32_t b = f2bf(f);
-        w = (i & 1) ? ((w & 0xffffu) | (b << 16)) : ((w & 0xffff0000u) | b);
-    }
+    __device__ __forceinline__ void put(const float (&f)[4]) { v = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])); }
+};
+template <> struct Raw<bf16, 2> {
+    uint32_t v;
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i ? (v & 0xffff0000u) : (v << 16)); }
+    __device__ __forceinline__ void put(const float (&f)[2]) { v = pack_bf16x2(f[0], f[1]); }
 };
 template <> struct Raw<bf16, 1> {
     unsigned short v;
     __device__ __forceinline__ float get(int) const { return bf2f(v); }
-    __device__ __forceinline__ void set(int, float f) { v = f2bf(f); }
+    __device__ __forceinline__ void put(const float (&f)[1]) { v = f2bf(f[0]); }
 };
 template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> ldr(const T* p) {
     Raw<T, VEC> r;
@@ -52,22 +59,24 @@ template <typename T, int VEC> __device__ __forceinline__ void str(T* p, const R
     *reinterpret_cast<decltype(r.v)*>(p) = r.v;
 }
 
-// a = sigmoid(f) and i = 1 - a, both to the last bits: the smaller of the two from the exponential, the larger as one
-// minus it.  fp32: the rounding of |f| log2(e) is carried along (|f| up to 80 would lose 6 bits); bf16 does not show it.
+// a = sigmoid(f) and i = 1 - a = sigmoid(-f), both to the last bits, from e = exp(-f): 1 / (1 + e) and e / (1 + e).  e is
+// held below 2^126 (no inf * 0); NaN passes.  fp32: the rounding of f log2(e) is carried along (|f| up to 80 would lose 6
+// bits); bf16 does not show it.
 template <typename T> __device__ __forceinline__ void gate(float f, float& a, float& i) {
-    float m = fabsf(f), e;
+    float e;
     if constexpr (sizeof(T) == 4) {
-        m = m > 127.f ? 127.f : m;                // infinities too; NaN stays
-        const float t = m * -1.4426950408889634f;
-        const float lo = fmaf(m, -1.4426950408889634f, -t) + m * -1.925963033500e-8f;
+        f = f < -87.f ? -87.f : f;
+        f = f > 104.f ? 104.f : f;
+        const float t = f * -1.4426950408889634f;
+        const float lo = fmaf(f, -1.4426950408889634f, -t) + f * -1.925963033500e-8f;
         e = __builtin_amdgcn_exp2f(t);
         e = fmaf(e * 0.6931471805599453f, lo, e);
     } else {
-        e = __builtin_amdgcn_exp2f(m * -1.4426950408889634f);
+        const float t = f * -1.4426950408889634f;
+        e = __builtin_amdgcn_exp2f(t > 126.f ? 126.f : t);
     }
-    const float sm = e * __builtin_amdgcn_rcpf(1.0f + e), lg = 1.0f - sm;
-    a = f >= 0.f ? lg : sm;
-    i = f >= 0.f ? sm : lg;
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    i = e * a;
 }
 
 struct RecP {
@@ -101,6 +110,32 @@ template <int VEC, int TS> struct Place {
     }
     // logical step t (0 .. L-1, in the order of the recurrence) -> row; the rows behind an item's length stay in place
     __device__ __forceinline__ int row(const RecP& p, int t) const { return p.reverse && t < len ? len - 1 - t : t; }
+    // TC rows from logical step t on.  all: every one is live for every lane of the wave (one pointer that walks); otherwise
+    // dead rows read row 0 instead, whose values are not used
+    template <typename T> __device__ __forceinline__ void load(const RecP& p, const T* base, int64_t sl, int t, bool all, Raw<T, VEC> (&r)[TC]) const {
+        if (all) {
+            const T* q = base + (int64_t)row(p, t) * sl;
+            const int64_t step = p.reverse ? -sl : sl;
+#pragma unroll
+            for (int i = 0; i < TC; ++i) r[i] = ldr<T, VEC>(q + i * step);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TC; ++i) r[i] = ldr<T, VEC>(base + (int64_t)(t + i < len ? row(p, t + i) : 0) * sl);
+        }
+    }
+    template <typename T> __device__ __forceinline__ void store(const RecP& p, T* base, int t, int te, bool all, const Raw<T, VEC> (&r)[TC]) const {
+        if (!ok) return;
+        if (all) {
+            T* q = base + (int64_t)row(p, t) * p.D;
+            const int64_t step = p.reverse ? -p.D : p.D;
+#pragma unroll
+            for (int i = 0; i < TC; ++i) str<T, VEC>(q + i * step, r[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+                if (t + i < te) str<T, VEC>(base + (int64_t)row(p, t + i) * p.D, r[i]);
+        }
+    }
 };
 
 // Combines the TS time lanes' maps (A, H) of one column and returns the state that this lane starts from, given the
@@ -110,31 +145,23 @@ template <int VEC, int TS, bool BACK>
 __device__ __forceinline__ void combine(float (&A)[VEC], float (&H)[VEC], float (&carry)[VEC], float (&in)[VEC], int ts, int cl,
                                         float* tot) {
     constexpr int CL = NTH / TS, TW = 64 / CL, NW = NTH / 64;       // time lanes of a wave, waves
+    static_assert(TW == 2, "two time lanes a wave: one exchange between its halves");
     const int wave = threadIdx.x >> 6, tw = ts % TW, pt = BACK ? TW - 1 - tw : tw;
+    float ea[VEC], eh[VEC];                                          // the other half's map, where it comes first
 #pragma unroll
-    for (int o = 1; o < TW; o <<= 1) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float a = BACK ? __shfl_down(A[v], o * CL, 64) : __shfl_up(A[v], o * CL, 64);
-            const float h = BACK ? __shfl_down(H[v], o * CL, 64) : __shfl_up(H[v], o * CL, 64);
-            H[v] = pt >= o ? fmaf(A[v], h, H[v]) : H[v];
-            A[v] = pt >= o ? A[v] * a : A[v];
-        }
+    for (int v = 0; v < VEC; ++v) {
+        const float a = __shfl_xor(A[v], 32, 64), h = __shfl_xor(H[v], 32, 64);
+        ea[v] = pt ? a : 1.f;
+        eh[v] = pt ? h : 0.f;
+        H[v] = fmaf(A[v], eh[v], H[v]);
+        A[v] *= ea[v];
     }
-    if (pt == TW - 1)
+    if (pt)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             tot[((wave * CL + cl) * 2 + 0) * VEC + v] = A[v];
             tot[((wave * CL + cl) * 2 + 1) * VEC + v] = H[v];
         }
-    float ea[VEC], eh[VEC];                                          // the lanes of this wave ahead of this one
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        const float a = BACK ? __shfl_down(A[v], CL, 64) : __shfl_up(A[v], CL, 64);
-        const float h = BACK ? __shfl_down(H[v], CL, 64) : __shfl_up(H[v], CL, 64);
-        ea[v] = pt ? a : 1.f;
-        eh[v] = pt ? h : 0.f;
-    }
     __syncthreads();
     float mine[VEC];
 #pragma unroll
@@ -157,6 +184,7 @@ __device__ __forceinline__ void fold_segments(const RecP& p, int64_t nd, const f
     for (int v = 0; v < VEC; ++v) c[v] = start ? start[nd + v] : 0.f;
     const int seg = blockIdx.y, cnt = BACK ? p.nseg - 1 - seg : seg;
     const int64_t ND = (int64_t)p.N * p.D;
+#pragma unroll 4
     for (int k = 0; k < cnt; ++k) {
         const float* g = p.agg + (int64_t)(BACK ? p.nseg - 1 - k : k) * 2 * ND + nd;
 #pragma unroll
@@ -168,39 +196,50 @@ __device__ __forceinline__ void fold_segments(const RecP& p, int64_t nd, const f
 // last step to its first, with dy in x's place.
 template <typename T, int VEC, int TS, bool BACK>
 __global__ __launch_bounds__(NTH) void rec_agg_kernel(const RecP p) {
-    constexpr int CL = NTH / TS, UN = 8;
+    constexpr int CL = NTH / TS;
     __shared__ float tot[NTH / 64 * CL * 2 * VEC];
     const Place<VEC, TS> w(p);
     const T* f = (const T*)p.f + (int64_t)(w.n / p.NI) * p.f_so + (int64_t)(w.n % p.NI) * p.f_si + w.d0;
     const T* x = BACK ? (const T*)p.dy + (int64_t)(w.n / p.NI) * p.g_so + (int64_t)(w.n % p.NI) * p.g_si + w.d0
                       : (const T*)p.x + (int64_t)(w.n / p.NI) * p.x_so + (int64_t)(w.n % p.NI) * p.x_si + w.d0;
     const int64_t xl = BACK ? p.g_sl : p.x_sl;
-    const int per = p.seg / TS, t0 = blockIdx.y * p.seg + w.ts * per, t1 = min(t0 + per, w.len);
+    const int per = p.seg / TS, nb = per / TC, t0 = blockIdx.y * p.seg + w.ts * per;      // (seg is a multiple of TS * TC)
     float A[VEC], H[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f;
-    for (int tb = t0; tb < t1; tb += UN) {
-        Raw<T, VEC> rf[UN], rx[UN];
+    Raw<T, VEC> rf[TC], rx[TC];
+    bool all = false;
+    auto load = [&](int k) {
+        const int t = t0 + (BACK ? nb - 1 - k : k) * TC;
+        all = __all(t + TC <= w.len);
+        if (__all(t >= w.len)) return;
+        w.load(p, f, p.f_sl, t, all, rf);
+        w.load(p, x, xl, t, all, rx);
+    };
+    load(0);
+    for (int k = 0; k < nb; ++k) {
+        const int t = t0 + (BACK ? nb - 1 - k : k) * TC;
+        const bool full = all;
+        Raw<T, VEC> cf[TC], cx[TC];
 #pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const int k = min(tb + i, t1 - 1), t = BACK ? t0 + t1 - 1 - k : k, r = w.row(p, t);
-            rf[i] = ldr<T, VEC>(f + (int64_t)r * p.f_sl);
-            rx[i] = ldr<T, VEC>(x + (int64_t)r * xl);
-        }
+        for (int i = 0; i < TC; ++i) cf[i] = rf[i], cx[i] = rx[i];
+        if (k + 1 < nb) load(k + 1);
+        if (__all(t >= w.len)) continue;
 #pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const bool on = tb + i < t1;
+        for (int j = 0; j < TC; ++j) {
+            const int i = BACK ? TC - 1 - j : j;
+            const bool on = full || t + i < w.len;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 float a, im;
-                gate<T>(rf[i].get(v), a, im);
-                const float h = BACK ? a * (rx[i].get(v) + H[v]) : fmaf(a, H[v], im * rx[i].get(v));
+                gate<T>(cf[i].get(v), a, im);
+                const float h = BACK ? a * (cx[i].get(v) + H[v]) : fmaf(a, H[v], im * cx[i].get(v));
                 H[v] = on ? h : H[v];
                 A[v] = on ? A[v] * a : A[v];
             }
         }
     }
-    // the whole segment's map: start from the two unit states (A: 1 -> with H's left out, H: 0)
+    // the whole segment's map: where the states 0 and (with H left out) 1 go
     float c[VEC], in[VEC], A2[VEC], H2[VEC], z[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) c[v] = 0.f, A2[v] = A[v], H2[v] = 0.f, z[v] = 1.f;
@@ -226,17 +265,18 @@ __global__ __launch_bounds__(NTH) void rec_fwd_kernel(const RecP p) {
     float c[VEC];
     fold_segments<VEC, false>(p, w.nd, p.h0, c);
     Raw<T, VEC> nx[TC], nf[TC];
+    bool all;
     auto load = [&](int tb) {
-#pragma unroll
-        for (int i = 0; i < TC; ++i) {
-            const int t = tb + w.ts * TC + i, r = t < w.len ? w.row(p, t) : 0;
-            nx[i] = ldr<T, VEC>(x + (int64_t)r * p.x_sl);
-            nf[i] = ldr<T, VEC>(f + (int64_t)r * p.f_sl);
-        }
+        const int t = tb + w.ts * TC;
+        all = __all(t + TC <= w.len);
+        w.load(p, x, p.x_sl, t, all, nx);
+        w.load(p, f, p.f_sl, t, all, nf);
     };
     load(ta);
     int buf = 0;
     for (int tb = ta; tb < te; tb += TILE) {
+        const int t = tb + w.ts * TC;
+        const bool full = all;
         if (p.st && tb > 0 && w.ok && w.ts == 0) {
             float* s = p.st + (int64_t)(tb / TILE) * p.N * p.D + w.nd;
 #pragma unroll
@@ -244,42 +284,50 @@ __global__ __launch_bounds__(NTH) void rec_fwd_kernel(const RecP p) {
         }
         float a[TC][VEC], b[TC][VEC], A[VEC], H[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f;
-#pragma unroll
-        for (int i = 0; i < TC; ++i) {
-            const bool live = tb + w.ts * TC + i < w.len;
+        for (int i = 0; i < TC; ++i)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                float im;
-                gate<T>(nf[i].get(v), a[i][v], im);
-                a[i][v] = live ? a[i][v] : 1.f;                 // padding: the state passes
-                b[i][v] = live ? im * nx[i].get(v) : 0.f;
-                if constexpr (TS > 1) {
+                gate<T>(nf[i].get(v), a[i][v], b[i][v]);
+                b[i][v] *= nx[i].get(v);
+            }
+        if (tb + TILE < te) load(tb + TILE);
+        if (!full)
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {                       // padding: the state passes
+                    a[i][v] = t + i < w.len ? a[i][v] : 1.f;
+                    b[i][v] = t + i < w.len ? b[i][v] : 0.f;
+                }
+        float h[VEC];
+        if constexpr (TS > 1) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) A[v] = a[0][v], H[v] = b[0][v];
+#pragma unroll
+            for (int i = 1; i < TC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
                     H[v] = fmaf(a[i][v], H[v], b[i][v]);
                     A[v] *= a[i][v];
                 }
-            }
-        }
-        if (tb + TILE < te) load(tb + TILE);
-        float h[VEC];
-        if constexpr (TS > 1) {
             combine<VEC, TS, false>(A, H, c, h, w.ts, w.cl, tot[buf]);
             buf ^= 1;
         } else {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) h[v] = c[v];
         }
+        Raw<T, VEC> o[TC];
 #pragma unroll
         for (int i = 0; i < TC; ++i) {
-            const int t = tb + w.ts * TC + i;
-            Raw<T, VEC> o;
+            float out[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 h[v] = fmaf(a[i][v], h[v], b[i][v]);
-                o.set(v, t < w.len ? h[v] : 0.f);
+                out[v] = full || t + i < w.len ? h[v] : 0.f;
             }
-            if (w.ok && t < te) str<T, VEC>(y + (int64_t)w.row(p, t) * p.D, o);
+            o[i].put(out);
         }
+        w.store(p, y, t, te, full, o);
         if constexpr (TS == 1)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) c[v] = h[v];
@@ -304,44 +352,55 @@ __global__ __launch_bounds__(NTH) void rec_bwd_kernel(const RecP p) {
     fold_segments<VEC, true>(p, w.nd, p.dlast, s);
     Raw<T, VEC> nx[TC], nf[TC], ng[TC];
     float nc[VEC];
+    bool all;
     auto load = [&](int tb) {
-#pragma unroll
-        for (int i = 0; i < TC; ++i) {
-            const int t = tb + w.ts * TC + i, r = t < w.len ? w.row(p, t) : 0;
-            nx[i] = ldr<T, VEC>(x + (int64_t)r * p.x_sl);
-            nf[i] = ldr<T, VEC>(f + (int64_t)r * p.f_sl);
-            ng[i] = ldr<T, VEC>(dy + (int64_t)r * p.g_sl);
-        }
+        const int t = tb + w.ts * TC;
+        all = __all(t + TC <= w.len);
+        w.load(p, x, p.x_sl, t, all, nx);
+        w.load(p, f, p.f_sl, t, all, nf);
+        w.load(p, dy, p.g_sl, t, all, ng);
         const float* st = tb > 0 ? p.st + (int64_t)(tb / TILE) * p.N * p.D : p.h0;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) nc[v] = st ? st[w.nd + v] : 0.f;
     };
     const int tl = ta + (te - ta - 1) / TILE * TILE;
     load(tl);
-    int buf = 0;
     for (int tb = tl; tb >= ta; tb -= TILE) {
+        const int t = tb + w.ts * TC;
+        const bool full = all;
+        // im: 1 - a; d: x, then h_{t-1} - x; g: dy
         float a[TC][VEC], im[TC][VEC], d[TC][VEC], g[TC][VEC], A[VEC], H[VEC], c[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f, c[v] = nc[v];
 #pragma unroll
-        for (int i = 0; i < TC; ++i) {
-            const bool live = tb + w.ts * TC + i < w.len;
+        for (int i = 0; i < TC; ++i)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 gate<T>(nf[i].get(v), a[i][v], im[i][v]);
-                a[i][v] = live ? a[i][v] : 1.f;
-                im[i][v] = live ? im[i][v] : 0.f;
-                d[i][v] = live ? nx[i].get(v) : 0.f;                  // x, then h_{t-1} - x
-                g[i][v] = live ? ng[i].get(v) : 0.f;
-                if constexpr (TS > 1) {
+                d[i][v] = nx[i].get(v);
+                g[i][v] = ng[i].get(v);
+            }
+        if (tb > ta) load(tb - TILE);
+        if (!full)
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const bool live = t + i < w.len;
+                    a[i][v] = live ? a[i][v] : 1.f;
+                    im[i][v] = live ? im[i][v] : 0.f;
+                    d[i][v] = live ? d[i][v] : 0.f;
+                    g[i][v] = live ? g[i][v] : 0.f;
+                }
+        float h[VEC];
+        if constexpr (TS > 1) {
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
                     H[v] = fmaf(a[i][v], H[v], im[i][v] * d[i][v]);
                     A[v] *= a[i][v];
                 }
-            }
-        }
-        if (tb > ta) load(tb - TILE);
-        float h[VEC];
-        if constexpr (TS > 1) {
             combine<VEC, TS, false>(A, H, c, h, w.ts, w.cl, tot[0]);
         } else {
 #pragma unroll
@@ -371,23 +430,22 @@ __global__ __launch_bounds__(NTH) void rec_bwd_kernel(const RecP p) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) sn[v] = s[v];
         }
+        Raw<T, VEC> ox[TC], of[TC];
 #pragma unroll
         for (int i = TC - 1; i >= 0; --i) {
-            const int t = tb + w.ts * TC + i;
-            Raw<T, VEC> ox, of;
+            float vx[VEC], vf[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float gt = g[i][v] + sn[v], gx = im[i][v] * gt;
-                ox.set(v, gx);                                        // (0 behind the length: im = 0)
-                of.set(v, gx * a[i][v] * d[i][v]);
+                const float gt = g[i][v] + sn[v];
                 sn[v] = a[i][v] * gt;
+                vx[v] = im[i][v] * gt;                                // (0 behind the length: im = 0)
+                vf[v] = im[i][v] * d[i][v] * sn[v];
             }
-            if (w.ok && t < te) {
-                const int64_t r = (int64_t)w.row(p, t) * p.D;
-                str<T, VEC>(dx + r, ox);
-                str<T, VEC>(df + r, of);
-            }
+            ox[i].put(vx);
+            of[i].put(vf);
         }
+        w.store(p, dx, t, te, full, ox);
+        w.store(p, df, t, te, full, of);
         if constexpr (TS == 1)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) s[v] = sn[v];
@@ -406,29 +464,28 @@ __global__ __launch_bounds__(NTH) void rec_step_kernel(const T* __restrict__ x, 
     const Raw<T, VEC> rx = ldr<T, VEC>(x + n * xs + d), rf = ldr<T, VEC>(f + n * fs + d);
     Raw<float, VEC> h = ldr<float, VEC>(st + n * D + d);
     Raw<T, VEC> o;
+    float hv[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
         float a, i;
         gate<T>(rf.get(v), a, i);
-        const float hv = fmaf(a, h.get(v), i * rx.get(v));
-        h.set(v, hv);
-        o.set(v, hv);
+        hv[v] = fmaf(a, h.get(v), i * rx.get(v));
     }
+    h.put(hv);
+    o.put(hv);
     str<float, VEC>(st + n * D + d, h);
     str<T, VEC>(y + n * D + d, o);
 }
 
-constexpr int TSPLIT = 16;                       // time lanes of the split form
-
 // How a call is cut: one time lane per column where the columns alone give every CU its eight waves (a tile then is TC
-// steps), else 16 time lanes; and, while that leaves fewer than four workgroups a CU, segments of the time axis whose
-// maps a first launch folds.
+// steps), else 8 time lanes; and, while that leaves fewer than four workgroups a CU, segments of the time axis whose maps
+// a first launch folds.
 struct Plan { int ts, vec, nseg, seg, tiles; int64_t cols, groups; };
 Plan plan_of(int64_t N, int L, int D, bool wide) {
     Plan q;
-    q.vec = wide ? 4 : 1;
+    q.vec = wide ? 2 : 1;
     q.cols = N * ((D + q.vec - 1) / q.vec);
-    q.ts = N * ((D + 3) / 4) >= 256 * 8 * 64 ? 1 : TSPLIT;    // (not by vec: the backward call has to cut the tiles as its forward did)
+    q.ts = N * ((D + 1) / 2) >= 256 * 8 * 64 ? 1 : TSPLIT;    // (not by vec: the backward call has to cut the tiles as its forward did)
     const int tile = q.ts * TC;
     q.tiles = (L + tile - 1) / tile;
     const int CL = NTH / q.ts;
@@ -443,7 +500,7 @@ Plan plan_of(int64_t N, int L, int D, bool wide) {
     return q;
 }
 
-// VEC = 4 needs every row of every operand on a 4-element boundary
+// VEC = 2 needs every row of every operand on a 2-element boundary
 bool is_wide(const DttRecurrence* g) {
     const int e = g->dtype ? 2 : 4;
     int64_t s = g->D;                             // (strides of axes of one element do not count)
@@ -451,7 +508,7 @@ bool is_wide(const DttRecurrence* g) {
     if (g->NI > 1) s |= g->x_si | g->f_si | g->g_si;
     if (g->L > 1) s |= g->x_sl | g->f_sl | g->g_sl;
     const uintptr_t a = (uintptr_t)g->x | (uintptr_t)g->f | (uintptr_t)g->dy | (uintptr_t)g->y | (uintptr_t)g->dx | (uintptr_t)g->df;
-    return s % 4 == 0 && a % (4 * e) == 0;
+    return s % 2 == 0 && a % (2 * e) == 0;
 }
 int fill(RecP& p, const DttRecurrence* g, Plan& q, const char* what) {
     DTT_CHECK(g, "%s: null argument", what);
@@ -490,10 +547,10 @@ template <typename T, int VEC, int TS> void launch_bwd(const RecP& p, const Plan
 #define REC_DISPATCH(FN)                                                                                                   \
     do {                                                                                                                   \
         if (g->dtype == 0) {                                                                                               \
-            if (q.vec == 4) { if (q.ts == 1) FN<float, 4, 1>(p, q, s); else FN<float, 4, TSPLIT>(p, q, s); }               \
+            if (q.vec == 2) { if (q.ts == 1) FN<float, 2, 1>(p, q, s); else FN<float, 2, TSPLIT>(p, q, s); }               \
             else { if (q.ts == 1) FN<float, 1, 1>(p, q, s); else FN<float, 1, TSPLIT>(p, q, s); }                          \
         } else {                                                                                                           \
-            if (q.vec == 4) { if (q.ts == 1) FN<bf16, 4, 1>(p, q, s); else FN<bf16, 4, TSPLIT>(p, q, s); }                 \
+            if (q.vec == 2) { if (q.ts == 1) FN<bf16, 2, 1>(p, q, s); else FN<bf16, 2, TSPLIT>(p, q, s); }                 \
             else { if (q.ts == 1) FN<bf16, 1, 1>(p, q, s); else FN<bf16, 1, TSPLIT>(p, q, s); }                            \
         }                                                                                                                  \
     } while (0)
