@@ -150,6 +150,16 @@ __device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32
         }
 }
 
+// The value of lane ^ 32 combined with this lane's: one exchange of the register file's halves (no LDS round trip)
+__device__ __forceinline__ float both_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Raw scores x of 32 NX keys -> weights 2^(sc x - m), with the running reference m and sum l of this lane's query.  The
 // reference need not be the maximum: it follows it only when a row's maximum has grown by more than 2^8 over it (weights up
 // to 256 keep all their relative precision in fp32 and bf16), so that the accumulators are hardly ever rescaled.
@@ -160,7 +170,7 @@ __device__ __forceinline__ void softmax_tile(f32x16_t (&x)[NX], float& m, float&
     for (int n = 0; n < NX; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+    top = both_max(top) * sc;
     if (__any(top > m + 8.f)) {
         const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         l *= al;
@@ -209,6 +219,21 @@ template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0
     return t;
 }
 
+// Scores of the keys j0 + acc_row(r, 0) that the query at pos does not see -> -inf.  The window is one comparison of the
+// distance from its first key; tiles with first tokens add theirs.
+__device__ __forceinline__ void hide_keys(const WaP& p, f32x16_t& x, int j0, int pos, int klen) {
+    const int lo = pos - p.left, hi = min(pos + p.right, klen - 1);
+    const uint32_t at = (uint32_t)(j0 - lo), span = (uint32_t)max(0, hi - lo + 1);
+    if (j0 < p.sinks) {
+        const int s = min(p.sinks - 1, hi) - j0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = at + acc_row(r, 0) < span || acc_row(r, 0) <= s ? x[r] : -INFINITY;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = at + acc_row(r, 0) < span ? x[r] : -INFINITY;
+    }
+}
+
 // RG row groups of 32 a workgroup, each by SP waves that take its 32-key tiles in turn and join at the end
 template <typename T, int DH, int RG, int SP>
 __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(const WaP p) {
@@ -217,8 +242,6 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     constexpr int BM = 32 * RG, NX = 1;
     __shared__ __align__(16) T img[2 * BN * I::LD];
     __shared__ float ml[SP > 1 ? RG : 1][2][32];
-    T* ks = img;
-    T* vs = img + BN * I::LD;
     static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
     int id = xcd_order(blockIdx.x, gridDim.x);
@@ -242,23 +265,22 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
     const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
     Stage<T, DH, BN> sk(p.k_st), sv(p.v_st);
-    int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
-    if (count > 0) {
-        sk.load(kp, p.k_st, t * BN, klen);
-        sv.load(v, p.v_st, t * BN, klen);
-    }
+    T* ks = img;
+    T* vs = img + BN * I::LD;
+    auto load = [&](int n) {
+        const int r0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
+        sk.load(kp, p.k_st, r0, klen);
+        sv.load(v, p.v_st, r0, klen);
+    };
+    if (count > 0) load(0);
     for (int n = 0; n < count; ++n) {
         __syncthreads();
         sk.store(ks);
         sv.store(vs);
         __syncthreads();
-        const int j0 = t * BN;
-        t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
-        if (n + 1 < count) {
-            sk.load(kp, p.k_st, t * BN, klen);
-            sv.load(v, p.v_st, t * BN, klen);
-        }
+        const int j0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
+        if (n + 1 < count) load(n + 1);
 #pragma unroll
         for (int k = 0; k < BN / 32 / SP; ++k) {
             const int sub = k * SP + sp, ja = j0 + 32 * sub, jb = ja + 31;
@@ -273,13 +295,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
                 for (int n = 0; n < NX; ++n) MM<T>::mma(nat_frag<T, DH>(ks, 32 * (sub + n) + lr, c, lh), qf[c], x[n]);
             if (!(jb <= pw + p.right && (ja >= pw + 31 - p.left || jb < p.sinks) && jb < klen)) {
 #pragma unroll
-                for (int n = 0; n < NX; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = ja + 32 * n + acc_row(r, lh);
-                        const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
-                        x[n][r] = see ? x[n][r] : -INFINITY;
-                    }
+                for (int n = 0; n < NX; ++n) hide_keys(p, x[n], ja + 32 * n + 4 * lh, pos, klen);
             }
             softmax_tile<DH, NX>(x, m, l, o, sc);
 #pragma unroll
@@ -292,7 +308,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
                 }
         }
     }
-    l += __shfl_xor(l, 32, 64);
+    l = both_sum(l);
     if constexpr (SP > 1) {
         float* at = reinterpret_cast<float*>(img) + rg * DH * 32;
         __syncthreads();
@@ -326,8 +342,6 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     typedef typename MM<T>::Frag Frag;
     constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
     __shared__ __align__(16) T img[2 * BN * I::LD];
-    T* ks = img;
-    T* vs = img + BN * I::LD;
     static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
     int id = xcd_order(blockIdx.x, gridDim.x);
@@ -354,7 +368,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
 #pragma unroll
         for (int e = 0; e < 8; ++e) dd = fmaf(ldf(a + e), ldf(z + e), dd);
     }
-    dd += __shfl_xor(dd, 32, 64);
+    dd = both_sum(dd);
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
     const float lse = p.lse[at];
     if (live && lh == 0 && sp == 0) p.dd[at] = dd;
@@ -365,23 +379,22 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     const int p0 = p.offset + qt * BM, p1 = min(p.offset + min(qt * BM + BM, p.Tq), qlen) - 1;
     const Tiles tl = key_tiles<BN>(p, p0, p1, klen);
     Stage<T, DH, BN> sk(p.k_st), sv(p.v_st);
-    int t = tl.a > 0 ? 0 : tl.b;
     const int count = tl.a + tl.c - tl.b + 1;
-    if (count > 0) {
-        sk.load(kp, p.k_st, t * BN, klen);
-        sv.load(v, p.v_st, t * BN, klen);
-    }
+    T* ks = img;
+    T* vs = img + BN * I::LD;
+    auto load = [&](int n) {
+        const int r0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
+        sk.load(kp, p.k_st, r0, klen);
+        sv.load(v, p.v_st, r0, klen);
+    };
+    if (count > 0) load(0);
     for (int n = 0; n < count; ++n) {
         __syncthreads();
         sk.store(ks);
         sv.store(vs);
         __syncthreads();
-        const int j0 = t * BN;
-        t = n + 1 < tl.a ? n + 1 : tl.b + (n + 1 - tl.a);
-        if (n + 1 < count) {
-            sk.load(kp, p.k_st, t * BN, klen);
-            sv.load(v, p.v_st, t * BN, klen);
-        }
+        const int j0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
+        if (n + 1 < count) load(n + 1);
 #pragma unroll
         for (int k = 0; k < BN / 32 / SP; ++k) {
             const int s = k * SP + sp, js = j0 + 32 * s;
@@ -395,14 +408,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
                 MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
             }
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
-            if (!full) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = js + acc_row(r, lh);
-                    const bool see = j <= pos + p.right && (j >= pos - p.left || j < p.sinks) && j < klen;
-                    x[r] = see ? x[r] : -INFINITY;
-                }
-            }
+            if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * y[r];
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
@@ -477,6 +483,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
         if (kt * KM < p.sinks) r1 = min(qrows, p.edge);                  // (and no chunks: all rows)
     }
     const int j = kw + lr, jc = min(j, p.Tk - 1);
+    const uint32_t span = j >= klen ? 0u : j < p.sinks ? 0x7fffffffu : (uint32_t)(p.left + p.right + 1);
     const T* k = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
     Frag kf[KL ? 1 : DH / 16], vf[VL ? 1 : DH / 16];
@@ -544,13 +551,10 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
                 else MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
             }
             const bool full = kw + 31 <= pr + p.right && (kw >= pr + 31 - p.left || kw + 31 < p.sinks) && kw + 31 < klen;
-            if (!full) {
+            if (!full) {                          // rows p with j - right <= p <= j + left (a first token: no end), one comparison
+                const uint32_t at = (uint32_t)(pr + 4 * lh - (j - p.right));
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int pp = pr + acc_row(r, lh);
-                    const bool see = j <= pp + p.right && (j >= pp - p.left || j < p.sinks) && j < klen;
-                    x[r] = see ? x[r] : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r) x[r] = at + acc_row(r, 0) < span ? x[r] : -INFINITY;
             }
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
@@ -713,7 +717,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
             for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(img, 16 * c, 32 * ct), pf[c], o[ct]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // and its reads ahead of the next writes
     }
-    l += __shfl_xor(l, 32, 64);
+    l = both_sum(l);
     // the four waves' states into one: weights 2^(m_w - m), channels of a column summed over the waves through LDS
     if (lh == 0) ml[wave][0][lr] = m, ml[wave][1][lr] = l;
     __syncthreads();
@@ -754,6 +758,117 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
             float* w = p.part + (((bh * p.ngrp + grp) * p.nsplit + split) * 32 + c) * (DH + 2);
             w[d] = acc[e];
             if (d < 2) w[DH + d] = ml[0][d][c];
+        }
+    }
+}
+
+// The same in fp32 for at most 4 query heads a key head, by vector arithmetic: an fp32 matrix tile computes 32 columns for 8192
+// cycles per 32 keys of 128 channels however few heads there are, this some 1000 per head (one frame of one stream, 256
+// slots, 2 heads of 128: 18.6 -> 7.0 us).  A row lies across LP lanes of 16 bytes; every such group of lanes keeps a
+// softmax of its own over the rows it reads, and the groups of the eight waves join at the end.
+template <int DH, int G>
+__global__ __launch_bounds__(512) void wattn_step_few_kernel(const WsP p) {
+    constexpr int NW = 8, LP = DH <= 32 ? 8 : DH <= 64 ? 16 : 32, RW = 64 / LP, U = 8, KB = RW * U, NG = NW * RW;
+    __shared__ float acc[NG][G][DH];
+    __shared__ float ml[NG][G][2];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sub = lane / LP, d0 = lane % LP * 4;
+    const bool in = d0 < DH;
+    int id = blockIdx.x;
+    const int split = id % p.nsplit; id /= p.nsplit;
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const int64_t pos = p.pos[b];
+    const int M = p.S + p.W, dl = in ? d0 : 0;
+    const int valid = pos < 0 ? 0 : (int)min((int64_t)M, pos + 1), cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
+    const float* kn = (const float*)p.k + b * p.k_sb + hk * p.k_sh + dl;
+    const float* vn = (const float*)p.v + b * p.v_sb + hk * p.v_sh + dl;
+    float* kc = (float*)p.kc + b * p.kc_sb + hk * p.kc_sh + dl;
+    float* vc = (float*)p.vc + b * p.vc_sb + hk * p.vc_sh + dl;
+    const int s0 = split * p.per, s1 = min(valid, s0 + p.per);
+    if (cur >= s0 && cur < s0 + p.per && wave == 3 && sub == 0 && in) {
+        // the new token's rows; every reader of this slot takes them from k, v instead
+        *reinterpret_cast<float4*>(kc + (int64_t)cur * p.kc_st) = *reinterpret_cast<const float4*>(kn);
+        *reinterpret_cast<float4*>(vc + (int64_t)cur * p.vc_st) = *reinterpret_cast<const float4*>(vn);
+    }
+    const float sc = p.scale * LOG2E;
+    float4 q[G], o[G];
+    float m[G], l[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        q[g] = *reinterpret_cast<const float4*>((const float*)p.q + b * p.q_sb + (hk * G + g) * p.q_sh + dl);
+        if (!in) q[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+        q[g].x *= sc, q[g].y *= sc, q[g].z *= sc, q[g].w *= sc;
+        o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[g] = -INFINITY, l[g] = 0.f;
+    }
+    Vec16<float> nk[U], nv[U];
+    auto load = [&](int js) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = js + u * RW + sub;
+            nk[u] = ld16_pred<float>(j == cur ? kn : kc + (int64_t)j * p.kc_st, kn, j < s1);
+            nv[u] = ld16_pred<float>(j == cur ? vn : vc + (int64_t)j * p.vc_st, vn, j < s1);
+        }
+    };
+    int js = s0 + wave * KB;
+    if (js < s1) load(js);
+    for (; js < s1; js += NW * KB) {
+        Vec16<float> k[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = nk[u], v[u] = nv[u];
+        if (js + NW * KB < s1) load(js + NW * KB);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float x[U], top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float4 a = k[u].v;
+                x[u] = fmaf(a.w, q[g].w, fmaf(a.z, q[g].z, fmaf(a.y, q[g].y, a.x * q[g].x)));
+#pragma unroll
+                for (int w = 1; w < LP; w <<= 1) x[u] += __shfl_xor(x[u], w, 64);
+                x[u] = js + u * RW + sub < s1 ? x[u] : -INFINITY;
+                top = fmaxf(top, x[u]);
+            }
+            if (__any(top > m[g] + 8.f)) {                              // (see softmax_tile)
+                const float mn = fmaxf(m[g], top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[g] - mn);
+                m[g] = mn, l[g] *= al;
+                o[g].x *= al, o[g].y *= al, o[g].z *= al, o[g].w *= al;
+            }
+            const float mu = m[g] == -INFINITY ? 0.f : m[g];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float e = __builtin_amdgcn_exp2f(x[u] - mu);
+                l[g] += e;
+                o[g].x = fmaf(e, v[u].v.x, o[g].x), o[g].y = fmaf(e, v[u].v.y, o[g].y);
+                o[g].z = fmaf(e, v[u].v.z, o[g].z), o[g].w = fmaf(e, v[u].v.w, o[g].w);
+            }
+        }
+    }
+    const int grp = wave * RW + sub;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        if (in) *reinterpret_cast<float4*>(&acc[grp][g][d0]) = o[g];
+        if (d0 == 0) ml[grp][g][0] = m[g], ml[grp][g][1] = l[g];
+    }
+    __syncthreads();
+    const int64_t bh = (int64_t)b * p.Hk + hk;
+    for (int e = threadIdx.x; e < G * DH; e += NW * 64) {
+        const int g = e / DH, d = e % DH;
+        float mt = -INFINITY, lt = 0.f, ot = 0.f;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mt = fmaxf(mt, ml[n][g][0]);
+        const float mu = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            const float w = __builtin_amdgcn_exp2f(ml[n][g][0] - mu);
+            lt = fmaf(ml[n][g][1], w, lt);
+            ot = fmaf(acc[n][g][d], w, ot);
+        }
+        if (p.nsplit == 1) {
+            ((float*)p.out)[((int64_t)b * p.Hq + hk * G + g) * DH + d] = lt != 0.f ? ot / lt : 0.f;
+        } else {
+            float* w = p.part + ((bh * p.nsplit + split) * 32 + g) * (DH + 2);
+            w[d] = ot;
+            if (d < 2) w[DH + d] = d ? lt : mt;
         }
     }
 }
@@ -969,7 +1084,16 @@ extern "C" int dtt_wattn_step(const DttWattnStep* g, void* stream) {
     DTT_CHECK(grid < (1ll << 31) && n < (1ll << 38), "dtt_wattn_step: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define STEP(T, D) hipLaunchKernelGGL((wattn_step_kernel<T, D>), dim3((unsigned)grid), dim3(NTH), 0, s, p)
-    WA_DISPATCH(STEP);
+#define FEW1(D, N) hipLaunchKernelGGL((wattn_step_few_kernel<D, N>), dim3((unsigned)grid), dim3(512), 0, s, p)
+#define FEW(T, D)                                                                                                   \
+    do {                                                                                                            \
+        if (p.G == 1) FEW1(D, 1); else if (p.G == 2) FEW1(D, 2); else if (p.G == 3) FEW1(D, 3); else FEW1(D, 4);     \
+    } while (0)
+    if (g->dtype) WA_DH(STEP, bf16);
+    else if (p.G <= 4) WA_DH(FEW, float);
+    else WA_DH(STEP, float);
+#undef FEW
+#undef FEW1
 #undef STEP
     if (p.nsplit > 1) {
         const dim3 gj((unsigned)((n + NTH - 1) / NTH));

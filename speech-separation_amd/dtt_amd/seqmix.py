@@ -25,6 +25,7 @@ from ._lib import lib, check, stream_ptr, dtype_code, DttError, DttRecurrence, D
 
 F32, BF16, F64, I32, I64 = torch.float32, torch.bfloat16, torch.float64, torch.int32, torch.int64
 _device = torch._C._cuda_getDevice
+_ROWS = torch.contiguous_format
 
 
 # --------------------------------------------------------------------------- #
@@ -113,7 +114,7 @@ def _rec_forward(x, f, h0, reverse, lengths, keep):
         g.lengths = lengths.data_ptr()
     if h0 is not None:
         g.h0 = h0.data_ptr()
-    y = x.new_empty(shape)
+    y = torch.empty_like(x, memory_format=_ROWS)
     last = torch.empty(shape[:-2] + shape[-1:], dtype=F32, device=x.device)
     g.y, g.last = y.data_ptr(), last.data_ptr()
     lib_, ref, states = lib(), C.byref(g), None
@@ -206,7 +207,7 @@ def gated_recurrence_step(x, f, state):
         with torch.cuda.device(x.device):
             return gated_recurrence_step(x, f, state)
     N, D = x.shape
-    x, f, y = _inner(x), _inner(f), torch.empty((N, D), dtype=x.dtype, device=x.device)
+    x, f, y = _inner(x), _inner(f), torch.empty_like(x, memory_format=_ROWS)
     if N * D:
         check(lib().dtt_recurrence_step(C.c_void_p(x.data_ptr()), C.c_void_p(f.data_ptr()), C.c_void_p(state.data_ptr()),
                                         C.c_void_p(y.data_ptr()), N, D, C.c_int64(x.stride(0)), C.c_int64(f.stride(0)),
@@ -227,7 +228,7 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
     if lengths is not None:
         g.lengths = lengths.data_ptr()
-    out, lse = q.new_empty(q.shape), None
+    out, lse = torch.empty_like(q, memory_format=_ROWS), None
     g.out = out.data_ptr()
     if keep:
         lse = torch.empty((B, Hq, Tq), dtype=F32, device=q.device)
@@ -344,7 +345,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, sinks=0, scale=N
     if q.get_device() != _device():
         with torch.cuda.device(q.device):
             return window_attention_step(q, k, v, k_cache, v_cache, positions, sinks, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=_ROWS)
     if q.shape[0] == 0:
         return out
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
@@ -407,11 +408,11 @@ def rotary_frequencies(dim, base=10000.0, stretch=1.0, trained=None, blend=(1.0,
 
 def _rotate(q, k, g):
     """q and k (or None) [B, T, H, dh] -> turned copies, by the positions, frequencies and layout that `g` holds."""
-    qo, ko = q.new_empty(q.shape), None
+    qo, ko = torch.empty_like(q, memory_format=_ROWS), None
     g.q, g.qo, g.Hq = q.data_ptr(), qo.data_ptr(), q.shape[2]
     g.q_sb, g.q_st, g.q_sh, _ = q.stride()
     if k is not None:
-        ko = k.new_empty(k.shape)
+        ko = torch.empty_like(k, memory_format=_ROWS)
         g.k, g.ko, g.Hk = k.data_ptr(), ko.data_ptr(), k.shape[2]
         g.k_sb, g.k_st, g.k_sh, _ = k.stride()
     else:

@@ -419,7 +419,8 @@ def test_attention_empty():
 # one frame at a time
 # --------------------------------------------------------------------------- #
 STEP = [(1, 1, 1, 32, 1, 0), (2, 2, 1, 64, 5, 2), (3, 6, 2, 128, 130, 4), (2, 40, 1, 32, 33, 0), (1, 8, 8, 96, 700, 16),
-        (2, 35, 1, 64, 1500, 3), (5, 4, 4, 128, 1024, 0), (1, 2, 2, 64, 3000, 1)]
+        (2, 35, 1, 64, 1500, 3), (5, 4, 4, 128, 1024, 0), (1, 2, 2, 64, 3000, 1),
+        (2, 9, 3, 128, 61, 2), (1, 4, 2, 32, 70, 0), (2, 8, 2, 96, 90, 1), (1, 5, 1, 64, 200, 0)]
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
