@@ -452,7 +452,8 @@ int dtt_clip_adamw_ex(const DttOptTensor* tab, int ntensors, const int32_t* chun
  * every item; last [N][D] (may be NULL) receives the state behind its last step.  states: dtt_recurrence_states() floats,
  * written by the forward call where not NULL and read by the backward call (same N, L, D, dtype and contents of x,
  * f, h0, lengths, reverse).  Backward: dy and dlast [N][D] (NULL: zero) in; dx, df and dh0 [N][D] (may be NULL) out.
- * ws: dtt_recurrence_ws_bytes() bytes for this call's pointers and strides (0: none needed), undefined afterwards. */
+ * ws: dtt_recurrence_ws_bytes() bytes for this call's pointers and strides, a backward call's where dy is set (0: none
+ * needed), undefined afterwards. */
 typedef struct {
     const void* x; const void* f; const void* dy;
     void* y; void* dx; void* df;

@@ -177,18 +177,31 @@ __device__ __forceinline__ void combine(float (&A)[VEC], float (&H)[VEC], float 
     for (int v = 0; v < VEC; ++v) in[v] = fmaf(ea[v], mine[v], eh[v]);
 }
 
-// state ahead of segment `seg` from the maps of the segments before it (BACK: behind it)
-template <int VEC, bool BACK>
-__device__ __forceinline__ void fold_segments(const RecP& p, int64_t nd, const float* start, float (&c)[VEC]) {
+// State ahead of this segment from the maps of the segments before it (BACK: behind it): every time lane folds a part of
+// them, in a few round trips to memory, and the parts are combined like a tile's (one thread after the other through 118
+// segments took 9 of the 48 us of an fp32 forward pass over 37501 x 512).
+template <int VEC, int TS, bool BACK>
+__device__ __forceinline__ void fold_segments(const RecP& p, int64_t nd, const float* start, float (&c)[VEC], int ts, int cl, float* tot) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) c[v] = start ? start[nd + v] : 0.f;
-    const int seg = blockIdx.y, cnt = BACK ? p.nseg - 1 - seg : seg;
-    const int64_t ND = (int64_t)p.N * p.D;
-#pragma unroll 4
-    for (int k = 0; k < cnt; ++k) {
-        const float* g = p.agg + (int64_t)(BACK ? p.nseg - 1 - k : k) * 2 * ND + nd;
+    if constexpr (TS > 1) {
+        const int cnt = BACK ? p.nseg - 1 - (int)blockIdx.y : (int)blockIdx.y;
+        if (cnt == 0) return;                                            // (the same for the whole workgroup)
+        const int64_t ND = (int64_t)p.N * p.D;
+        const int per = (cnt + TS - 1) / TS, k0 = (BACK ? TS - 1 - ts : ts) * per, k1 = min(cnt, k0 + per);
+        float A[VEC], H[VEC], in[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) c[v] = fmaf(g[v], c[v], g[ND + v]);
+        for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f;
+#pragma unroll 4
+        for (int k = k0; k < k1; ++k) {
+            const float* g = p.agg + (int64_t)(BACK ? p.nseg - 1 - k : k) * 2 * ND + nd;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                H[v] = fmaf(g[v], H[v], g[ND + v]);
+                A[v] *= g[v];
+            }
+        }
+        combine<VEC, TS, BACK>(A, H, c, in, ts, cl, tot);
     }
 }
 
@@ -263,7 +276,7 @@ __global__ __launch_bounds__(NTH) void rec_fwd_kernel(const RecP p) {
     T* y = (T*)p.y + (int64_t)w.n * p.L * p.D + w.d0;
     const int ta = blockIdx.y * p.seg, te = min(p.L, ta + p.seg);
     float c[VEC];
-    fold_segments<VEC, false>(p, w.nd, p.h0, c);
+    fold_segments<VEC, TS, false>(p, w.nd, p.h0, c, w.ts, w.cl, tot[1]);
     Raw<T, VEC> nx[TC], nf[TC];
     bool all;
     auto load = [&](int tb) {
@@ -349,7 +362,7 @@ __global__ __launch_bounds__(NTH) void rec_bwd_kernel(const RecP p) {
     T* df = (T*)p.df + (int64_t)w.n * p.L * p.D + w.d0;
     const int ta = blockIdx.y * p.seg, te = min(p.L, ta + p.seg);
     float s[VEC];                                                    // s_{t+1} of the step behind the tile
-    fold_segments<VEC, true>(p, w.nd, p.dlast, s);
+    fold_segments<VEC, TS, true>(p, w.nd, p.dlast, s, w.ts, w.cl, tot[1]);
     Raw<T, VEC> nx[TC], nf[TC], ng[TC];
     float nc[VEC];
     bool all;
@@ -477,29 +490,6 @@ __global__ __launch_bounds__(NTH) void rec_step_kernel(const T* __restrict__ x, 
     str<T, VEC>(y + n * D + d, o);
 }
 
-// How a call is cut: one time lane per column where the columns alone give every CU its eight waves (a tile then is TC
-// steps), else 8 time lanes; and, while that leaves fewer than four workgroups a CU, segments of the time axis whose maps
-// a first launch folds.
-struct Plan { int ts, vec, nseg, seg, tiles; int64_t cols, groups; };
-Plan plan_of(int64_t N, int L, int D, bool wide) {
-    Plan q;
-    q.vec = wide ? 2 : 1;
-    q.cols = N * ((D + q.vec - 1) / q.vec);
-    q.ts = N * ((D + 1) / 2) >= 256 * 8 * 64 ? 1 : TSPLIT;    // (not by vec: the backward call has to cut the tiles as its forward did)
-    const int tile = q.ts * TC;
-    q.tiles = (L + tile - 1) / tile;
-    const int CL = NTH / q.ts;
-    q.groups = (q.cols + CL - 1) / CL;
-    q.nseg = 1;
-    if (q.ts > 1) {
-        const int64_t want = 1024 / q.groups, most = q.tiles / 4;     // segments of four tiles at least
-        q.nseg = (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
-    }
-    q.seg = (q.tiles + q.nseg - 1) / q.nseg * tile;
-    q.nseg = (L + q.seg - 1) / q.seg;
-    return q;
-}
-
 // VEC = 2 needs every row of every operand on a 2-element boundary
 bool is_wide(const DttRecurrence* g) {
     const int e = g->dtype ? 2 : 4;
@@ -510,11 +500,38 @@ bool is_wide(const DttRecurrence* g) {
     const uintptr_t a = (uintptr_t)g->x | (uintptr_t)g->f | (uintptr_t)g->dy | (uintptr_t)g->y | (uintptr_t)g->dx | (uintptr_t)g->df;
     return s % 2 == 0 && a % (2 * e) == 0;
 }
+// How a call is cut: one time lane per column where the columns alone give every CU its eight waves (a tile then is TC
+// steps), else 8 time lanes; and, where that leaves CUs empty, segments of the time axis (of four tiles at least) whose maps
+// a first launch folds: as many as fill one round of resident workgroups.  Residence goes by registers: four workgroups a
+// CU forward, three backward (two in fp32); 30 segments instead of 24, a quarter into a second round, took 65 instead of
+// 57 us in a backward pass over 2 x 15001 x 1024.
+struct Plan { int ts, vec, nseg, seg, tiles; int64_t cols, groups; };
+Plan plan_of(const DttRecurrence* g) {
+    const int64_t N = g->N;
+    const int L = g->L, D = g->D, slots = g->dy ? g->dtype ? 768 : 512 : 1024;
+    Plan q;
+    q.vec = is_wide(g) ? 2 : 1;
+    q.cols = N * ((D + q.vec - 1) / q.vec);
+    q.ts = N * ((D + 1) / 2) >= 256 * 8 * 64 ? 1 : TSPLIT;    // (not by vec: the backward call has to cut the tiles as its forward did)
+    const int tile = q.ts * TC;
+    q.tiles = (L + tile - 1) / tile;
+    const int CL = NTH / q.ts;
+    q.groups = (q.cols + CL - 1) / CL;
+    q.nseg = 1;
+    if (q.ts > 1) {
+        const int64_t want = slots / q.groups, most = q.tiles / 4;
+        q.nseg = (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+    }
+    q.seg = (q.tiles + q.nseg - 1) / q.nseg * tile;
+    q.nseg = (L + q.seg - 1) / q.seg;
+    return q;
+}
+
 int fill(RecP& p, const DttRecurrence* g, Plan& q, const char* what) {
     DTT_CHECK(g, "%s: null argument", what);
     DTT_CHECK(g->N > 0 && g->L > 0 && g->D > 0 && g->NI > 0 && g->N % g->NI == 0, "%s: bad sizes N=%d NI=%d L=%d D=%d", what, g->N,
               g->NI, g->L, g->D);
-    q = plan_of(g->N, g->L, g->D, is_wide(g));
+    q = plan_of(g);
     DTT_CHECK(g->L <= (1 << 30), "%s: L=%d, at most 2^30", what, g->L);
     DTT_CHECK(g->dtype == 0 || g->dtype == 1, "%s: dtype must be 0 (float32) or 1 (bfloat16)", what);
     DTT_CHECK(g->x && g->f, "%s: null buffer", what);
@@ -558,13 +575,13 @@ template <typename T, int VEC, int TS> void launch_bwd(const RecP& p, const Plan
 
 extern "C" int64_t dtt_recurrence_ws_bytes(const DttRecurrence* g) {
     if (!g || g->N <= 0 || g->L <= 0 || g->D <= 0) return 0;
-    const Plan q = plan_of(g->N, g->L, g->D, is_wide(g));
+    const Plan q = plan_of(g);
     return q.nseg > 1 ? (int64_t)q.nseg * 2 * g->N * g->D * 4 : 0;
 }
 
 extern "C" int64_t dtt_recurrence_states(const DttRecurrence* g) {
     if (!g || g->N <= 0 || g->L <= 0 || g->D <= 0) return 0;
-    return (int64_t)plan_of(g->N, g->L, g->D, is_wide(g)).tiles * g->N * g->D;
+    return (int64_t)plan_of(g).tiles * g->N * g->D;
 }
 
 extern "C" int dtt_recurrence_fwd(const DttRecurrence* g, void* stream) {
