@@ -23,7 +23,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 struct WaP {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
-    void* out; void* dq; void* dk; void* dv;
+    void* out; void* lo; void* dq; void* dk; void* dv;
     float* lse; float* dd; float* part;
     const int* len;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
@@ -86,6 +86,13 @@ template <typename T> __device__ __forceinline__ typename MM<T>::Frag acc_frag(c
         f.hi = make_float4(s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]);
         return f;
     }
+}
+// what acc_frag's rounding leaves off registers 8 c .. 8 c + 7, as a fragment (bf16)
+__device__ __forceinline__ s16x8_t rest_frag(const f32x16_t& s, int c) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s[8 * c + e] - bf2f(f2bf(s[8 * c + e]));
+    return __builtin_bit_cast(s16x8_t, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
 }
 __device__ __forceinline__ f32x16_t zero_acc() {
     f32x16_t z;
@@ -206,6 +213,24 @@ template <int N> __device__ __forceinline__ void unpark(const float* at, f32x16_
         for (int r = 0; r < 16; ++r) a[c][r] = fmaf(at[(c * 16 + r) * 64 + lane], theirs, a[c][r] * mine);
 }
 
+// What store_rows' rounding to bf16 leaves off.  D = sum(dO O) from O as rounded would carry 2^-9 of |dO| |O| into every
+// dP - D of the row, as much again as dS's own rounding where a row sees few keys; with the rest of O beside it that is 2^-17.
+template <int DH>
+__device__ __forceinline__ void store_rest(bf16* row, const f32x16_t (&acc)[DH / 32], float mul, int lh) {
+#pragma unroll
+    for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float a = acc[ct][4 * q + e] * mul;
+                v[e] = a - bf2f(f2bf(a));
+            }
+            *reinterpret_cast<uint2*>(row + 32 * ct + 8 * q + 4 * lh) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        }
+}
+
 // The key tiles (of N keys) that the query rows at positions p0 .. p1 see: [0, a) holds first tokens only, [b, c] the window.
 struct Tiles { int a, b, c; };
 template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0, int p1, int klen) {
@@ -217,6 +242,13 @@ template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0
     if (jmin <= jmax) t.b = jmin / N, t.c = jmax / N, t.a = min(t.a, t.b);
     else t.b = t.a, t.c = t.a - 1;
     return t;
+}
+
+// How many keys the query at pos sees.  A softmax over one key is 1 whatever the score is: such a row has no gradient through
+// its weights, which dP - D would give only up to rounding.
+__device__ __forceinline__ int seen_keys(const WaP& p, int pos, int klen) {
+    const int hi = min(pos + p.right, klen - 1), lo = max(0, pos - p.left);
+    return max(0, hi - lo + 1) + max(0, min(min(p.sinks, lo), hi + 1));
 }
 
 // Scores of the keys j0 + acc_row(r, 0) that the query at pos does not see -> -inf.  The window is one comparison of the
@@ -326,12 +358,14 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     }
     if (i >= p.Tq) return;
     const bool live = pos < qlen && l != 0.f;         // (l is at least 1 where anything is visible; NaN passes)
-    T* out = (T*)p.out + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH;
+    T* out = (T*)p.out + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH;
     if (!live) {
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
     }
     store_rows<T, DH>(out, o, live ? 1.f / l : 0.f, lh);
+    if constexpr (sizeof(T) == 2)
+        if (p.lo) store_rest<DH>((bf16*)p.lo + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH, o, live ? 1.f / l : 0.f, lh);
     if (p.lse && lh == 0) p.lse[((int64_t)b * p.Hq + h) * p.Tq + i] = live ? m + log2f(l) : INFINITY;
 }
 
@@ -341,6 +375,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
+    constexpr bool FINE = sizeof(T) == 2 && SP == 2;           // dS in two bf16 pieces, see fine()
     __shared__ __align__(16) T img[2 * BN * I::LD];
     static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
@@ -353,22 +388,31 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     const bool live = i < p.Tq && pos < qlen;
     const T* q = (const T*)p.q + b * p.q_sb + (int64_t)ic * p.q_st + h * p.q_sh;
     const T* go = (const T*)p.dout + b * p.g_sb + (int64_t)ic * p.g_st + h * p.g_sh;
-    const T* oo = (const T*)p.o + ((int64_t)(b * p.Tq + ic) * p.Hq + h) * DH;
+    const T* oo = (const T*)p.o + (((int64_t)b * p.Tq + ic) * p.Hq + h) * DH;
     const T* kp = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
     Frag qf[DH / 16], gf[DH / 16];
-    float dd = 0.f;
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c) {
         qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
         gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
-        const T* a = reinterpret_cast<const T*>(&gf[c]);
-        const Frag of = MM<T>::ldfrag(oo + 16 * c + 8 * lh);
-        const T* z = reinterpret_cast<const T*>(&of);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dd = fmaf(ldf(a + e), ldf(z + e), dd);
     }
-    dd = both_sum(dd);
+    // D by the matrix cores, as the diagonal of O dO^T
+    float dd = 0.f;
+    {
+        f32x16_t t = zero_acc();
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) MM<T>::mma(MM<T>::ldfrag(oo + 16 * c + 8 * lh), gf[c], t);
+        if constexpr (sizeof(T) == 2)
+            if (p.lo) {
+                const T* lo = (const T*)p.lo + (oo - (const T*)p.o) + 8 * lh;
+#pragma unroll
+                for (int c = 0; c < DH / 16; ++c) MM<T>::mma(MM<T>::ldfrag(lo + 16 * c), gf[c], t);
+            }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dd += acc_row(r, lh) == lr ? t[r] : 0.f;
+        dd = both_sum(dd);
+    }
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
     const float lse = p.lse[at];
     if (live && lh == 0 && sp == 0) p.dd[at] = dd;
@@ -399,9 +443,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         for (int k = 0; k < BN / 32 / SP; ++k) {
             const int s = k * SP + sp, js = j0 + 32 * s;
             if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
-            f32x16_t x = zero_acc(), y;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) y[r] = -dd;                      // y = dP - D
+            f32x16_t x = zero_acc(), y = zero_acc();
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
                 MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
@@ -410,12 +452,16 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
             if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * y[r];
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * (y[r] - dd);
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int ct = 0; ct < DH / 32; ++ct) MM<T>::mma(tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct), pf[c], dq[ct]);
+                for (int ct = 0; ct < DH / 32; ++ct) {
+                    const Frag kt = tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct);
+                    MM<T>::mma(kt, pf[c], dq[ct]);
+                    if constexpr (FINE) MM<T>::mma(kt, rest_frag(x, c), dq[ct]);
+                }
         }
     }
     if constexpr (SP > 1) {
@@ -427,11 +473,11 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         unpark(mem, dq, lane, 1.f, 1.f);
     }
     if (i >= p.Tq) return;
-    if (!live || lse == INFINITY) {
+    if (!live || seen_keys(p, pos, klen) <= 1) {
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
     }
-    store_rows<T, DH>((T*)p.dq + ((int64_t)(b * p.Tq + i) * p.Hq + h) * DH, dq, p.scale, lh);
+    store_rows<T, DH>((T*)p.dq + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH, dq, p.scale, lh);
 }
 
 // dk, dv: a workgroup owns 32 KG keys of one key head (32 a wave) and walks the query rows that see them, over the heads of
@@ -447,12 +493,13 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     // V's fragments (and K's) are read from LDS where with both sums, both tiles and the next rows on their way they would
     // exceed the registers of two waves a SIMD (fp32: of one)
     constexpr int KM = 32 * KG, NT = KG * SP * 64;
+    constexpr bool FINE = sizeof(T) == 2 && KG == 2;           // dS in two bf16 pieces, see fine()
     constexpr bool VL = DH >= 96, KL = DH == 128 && sizeof(T) == 2 && KG * SP == 8;
     constexpr int TILE = QN * I::LD, OWN = KM * I::LD, N = 2 * TILE + (VL ? OWN : 0) + (KL ? OWN : 0);
     constexpr int PARK = SP > 1 ? KG * DH * 128 / (int)sizeof(T) : 0;
     static_assert(SP <= QN / 32, "a 32-row tile of a staged one for every wave that shares keys");
     __shared__ __align__(16) T mem[N > PARK ? N : PARK];
-    __shared__ __align__(16) float st[2][QN];
+    __shared__ __align__(16) float st[3][QN];     // per row: log of the sum, D, and 1 (0 where one key is seen: no gradient of weights)
     T* qs = mem;
     T* gs = mem + TILE;
     T* vimg = mem + 2 * TILE;
@@ -506,7 +553,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     const float sc = p.scale * LOG2E;
     Stage<T, DH, QN, NT> sq(p.q_st), sg(p.g_st);
     const int per = r1 > r0 ? (r1 - r0 + QN - 1) / QN : 0, count = per * p.G;
-    float sl = 0.f, sd = 0.f;
+    float sl = 0.f, sd = 0.f, sw = 0.f;
     auto load = [&](int n) {
         const int h = hk * p.G + n / per, r = r0 + n % per * QN;
         sq.load((const T*)p.q + b * p.q_sb + h * p.q_sh, p.q_st, r, r1);
@@ -516,7 +563,8 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + min(i, p.Tq - 1);
             const float lv = p.lse[at], dvv = p.dd[at];
             sl = i < r1 ? lv : INFINITY;
-            sd = i < r1 ? dvv : 0.f;
+            sw = i < r1 && seen_keys(p, p.offset + i, klen) > 1 ? 1.f : 0.f;
+            sd = sw != 0.f ? dvv : 0.f;
         }
     };
     if (count > 0) load(0);
@@ -524,7 +572,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
         __syncthreads();
         sq.store(qs);
         sg.store(gs);
-        if (threadIdx.x < QN) st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd;
+        if (threadIdx.x < QN) st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd, st[2][threadIdx.x] = sw;
         __syncthreads();
         const int i0 = r0 + n % per * QN;
         if (n + 1 < count) load(n + 1);
@@ -534,12 +582,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             if (far && (it || wave >= QN / 32)) continue;
             const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
-            f32x16_t x = zero_acc(), y;
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const float4 ds = *reinterpret_cast<const float4*>(&st[1][32 * s + 8 * r4 + 4 * lh]);
-                y[4 * r4] = -ds.x, y[4 * r4 + 1] = -ds.y, y[4 * r4 + 2] = -ds.z, y[4 * r4 + 3] = -ds.w;     // y = dP - D
-            }
+            f32x16_t x = zero_acc(), y = zero_acc();
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
                 if constexpr (KL) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), nat_frag<T, DH>(kimg, vr, c, lh), x);
@@ -559,11 +602,13 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const float4 ls = *reinterpret_cast<const float4*>(&st[0][32 * s + 8 * r4 + 4 * lh]);
+                const float4 ds = *reinterpret_cast<const float4*>(&st[1][32 * s + 8 * r4 + 4 * lh]);
+                const float4 ws = *reinterpret_cast<const float4*>(&st[2][32 * s + 8 * r4 + 4 * lh]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * r4 + e;
                     x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(&ls.x)[e]));
-                    y[r] *= x[r];
+                    y[r] = x[r] * fmaf(y[r], (&ws.x)[e], -(&ds.x)[e]);
                 }
             }
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
@@ -573,7 +618,9 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     MM<T>::mma(tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct), pf[c], dv[ct]);
-                    MM<T>::mma(tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct), df[c], dk[ct]);
+                    const Frag qt = tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct);
+                    MM<T>::mma(qt, df[c], dk[ct]);
+                    if constexpr (FINE) MM<T>::mma(qt, rest_frag(y, c), dk[ct]);
                 }
         }
     }
@@ -599,7 +646,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
         store_rows<float, DH>(d + DH, dv, 1.f, lh);
     }
     if (far || j >= p.Tk || (p.nchunk > 0 && j < p.sinks)) return;
-    const int64_t row = ((int64_t)(b * p.Tk + j) * p.Hk + hk) * DH;
+    const int64_t row = (((int64_t)b * p.Tk + j) * p.Hk + hk) * DH;
     store_rows<T, DH>((T*)p.dk + row, dk, p.scale, lh);
     store_rows<T, DH>((T*)p.dv + row, dv, 1.f, lh);
 }
@@ -656,7 +703,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
     const int hk = id % p.Hk, b = id / p.Hk;
     const int64_t pos = p.pos[b];
     const int M = p.S + p.W;
-    const int valid = pos < 0 ? 0 : (int)min((int64_t)M, pos + 1), cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
+    const int valid = pos < 0 ? 0 : pos >= M ? M : (int)pos + 1, cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
     const int hg = grp * 32 + lr, h = hk * p.G + min(hg, p.G - 1);
     const T* q = (const T*)p.q + b * p.q_sb + h * p.q_sh;
     const T* kn = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
@@ -778,7 +825,7 @@ __global__ __launch_bounds__(512) void wattn_step_few_kernel(const WsP p) {
     const int hk = id % p.Hk, b = id / p.Hk;
     const int64_t pos = p.pos[b];
     const int M = p.S + p.W, dl = in ? d0 : 0;
-    const int valid = pos < 0 ? 0 : (int)min((int64_t)M, pos + 1), cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
+    const int valid = pos < 0 ? 0 : pos >= M ? M : (int)pos + 1, cur = pos < 0 ? -1 : slot_of(pos, p.S, p.W);
     const float* kn = (const float*)p.k + b * p.k_sb + hk * p.k_sh + dl;
     const float* vn = (const float*)p.v + b * p.v_sb + hk * p.v_sh + dl;
     float* kc = (float*)p.kc + b * p.kc_sb + hk * p.kc_sh + dl;
@@ -926,7 +973,7 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
     p = WaP{};
     p.q = g->q; p.k = g->k; p.v = g->v; p.o = g->out; p.out = g->out; p.dout = g->dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
-    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
+    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths; p.lo = g->dtype ? g->out_rest : nullptr;
     // (strides of axes of one element do not count)
     const bool b = g->B > 1, tq = g->Tq > 1, tk = g->Tk > 1, hq = g->Hq > 1, hk = g->Hk > 1;
     p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : g->DH; p.q_sh = hq ? g->q_sh : 0;
@@ -953,9 +1000,15 @@ void far_chunks(WaP& p) {
 }
 int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk * p.npart * p.sinks * 2 * dh * 4 : 0; }
 
-// Few rows: half of them a workgroup, two waves on each (the walk over its keys half as long).  512 workgroups are two a CU.
+// Few rows: half of them a workgroup, two waves on each (the walk over its keys half as long): fp32 training over 16 clips of
+// 376 frames, 2 heads of 128: forward 45 -> 24 us, dq 60 -> 34, dk / dv 85 -> 37; with 1024 workgroups, two to four a CU,
+// the other way: forward 69 -> 85 us at 2 x 4096 rows, 16 / 4 heads.  512 workgroups are two a CU.
 bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
 bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
+// Rows of few keys: the rounding of dS to bf16 (2^-9 of each) does not average out over two or three keys, and dq and dk come
+// out 1.5 to 1.6 times as far from the exact ones as their own rounding is; over 20 keys and more it is 1.4.  The kernels for few rows
+// carry what the rounding leaves off as a second operand (a third more matrix instructions); small windows take them too.
+bool fine(const WaP& p) { return (int64_t)p.left + p.right + p.sinks < 24; }
 
 #define WA_DH(FN, T)                                                              \
     do {                                                                          \
@@ -971,7 +1024,7 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     DTT_CHECK(g, "dtt_wattn_fwd: null argument");
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_fwd")) return rc;
-    DTT_CHECK(g->out && aligned16(g->out), "dtt_wattn_fwd: null or unaligned output");
+    DTT_CHECK(g->out && aligned16(g->out) && aligned16(g->out_rest), "dtt_wattn_fwd: null or unaligned output");
     const bool split = split_rows(p);
     const int bm = split ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
@@ -1001,14 +1054,14 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_bwd")) return rc;
     DTT_CHECK(g->out && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
-    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
+    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->out_rest) && aligned16(g->dout) && aligned16(g->dq) &&
               aligned16(g->dk) && aligned16(g->dv), "dtt_wattn_bwd: rows must start on 16 bytes");
     far_chunks(p);
     const int64_t need = part_bytes(p, g->DH);
     DTT_CHECK(need == 0 || (g->ws && aligned16(g->ws) && g->ws_bytes >= need), "dtt_wattn_bwd: workspace of %lld bytes, %lld given",
               (long long)need, (long long)g->ws_bytes);
     p.part = (float*)g->ws;
-    const bool split = split_rows(p), splitk = split_keys(p);
+    const bool split = split_rows(p) || fine(p), splitk = split_keys(p) || fine(p);
     const int bm = split ? 64 : 128, km = splitk ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
     WaP pk = p;

@@ -228,26 +228,29 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
     if lengths is not None:
         g.lengths = lengths.data_ptr()
-    out, lse = torch.empty_like(q, memory_format=_ROWS), None
+    out, lse, rest = torch.empty_like(q, memory_format=_ROWS), None, None
     g.out = out.data_ptr()
     if keep:
+        if q.dtype is BF16:
+            rest = torch.empty_like(out)
+            g.out_rest = rest.data_ptr()
         lse = torch.empty((B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
     check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
-    return out, lse, g
+    return out, lse, rest, g
 
 
 class WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, cfg):
-        out, lse, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
-        ctx.save_for_backward(q, k, v, lengths, out, lse)
+        out, lse, rest, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
+        ctx.save_for_backward(q, k, v, lengths, out, lse, rest)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, lengths, out, lse = ctx.saved_tensors
+        q, k, v, lengths, out, lse, rest = ctx.saved_tensors                  # (out, rest: alive; the struct has their addresses)
         do, g = _rows_attn(do), _again(ctx.call)
         dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse)
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
@@ -326,6 +329,9 @@ def _step_args(name, k, v, k_cache, v_cache, sinks, scale):
     g.kc, g.vc = k_cache.data_ptr(), v_cache.data_ptr()
     if ke != 1 or ve != 1 or (g.kc | g.vc) % 16 or (g.kc_sb | g.kc_st | g.kc_sh | g.vc_sb | g.vc_st | g.vc_sh) * k.element_size() % 16:
         _fail(name, "cache rows must be contiguous and start on 16 bytes")
+    if g.kc == g.vc or (cs[0] > 1 and not (g.kc_sb and g.vc_sb)) or (cs[1] > 1 and not (g.kc_st and g.vc_st)) or (
+            cs[2] > 1 and not (g.kc_sh and g.vc_sh)):
+        _fail(name, "every slot of every cache must have memory of its own (no broadcast caches)")
     return g
 
 

@@ -285,7 +285,8 @@ def attn_ref(q, k, v, see, scale, dt, do=None):
     dd = torch.where(rows, dd, 0.0)
     dP, mP = dd @ vd.transpose(-1, -2), dd.abs() @ vd.abs().transpose(-1, -2)
     D = (dd * o).sum(-1, keepdim=True)
-    eD = (dd.abs() * (eo + R(dt) * o.abs())).sum(-1, keepdim=True) + (dh + 4) * U * (dd.abs() * o.abs()).sum(-1, keepdim=True)
+    rest = 2.0 ** -16 if dt == BF else U                                    # (bfloat16: O and what its rounding left off)
+    eD = (dd.abs() * (eo + rest * o.abs())).sum(-1, keepdim=True) + (dh + 4) * U * (dd.abs() * o.abs()).sum(-1, keepdim=True)
     dS = P * (dP - D)
     mS = P * (dP - D).abs()
     eS = P * ((dh + 4) * U * mP + eD) + (w + 8 * U) * mS + rp * mS
@@ -406,6 +407,32 @@ def test_attention_gradient_against_differences():
         f = lambda a: float((attn_ref(*a, see, 32 ** -0.5, F32)[0][0] * do.double()).sum())  # noqa: E731
         num = (f(up) - f(dn)) / 2e-4
         assert abs(num - float((g[i].double() * d).sum())) <= 1e-5 * float(g[i].double().norm() * d.norm()) + 1e-6
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("T,left,dh", [(1, 5, 64), (1, 0, 128), (300, 0, 32), (90, 0, 96), (2000, 0, 128)])
+def test_attention_rows_of_one_key_have_no_gradient_through_their_weights(dt, T, left, dh):
+    """A softmax over one key is 1 whatever its score is: dq = dk = 0 exactly (o and dv, in float32, to the rounding of a
+    weight: an exponential of a score less its own log, 4 U and the 2 U |score| of the products, |score| below 32)."""
+    q, k, v = (rnd(s, 2, T, 2, dh, dt=dt, grad=True) for s in (1, 2, 3))
+    do = rnd(4, 2, T, 2, dh, dt=dt)
+    o = A().window_attention(q, k, v, left)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    assert not dq.any() and not dk.any()
+    for got, want in ((o, v.detach().double()), (dv, do.double())):
+        within(got, want, (70 * U + R(dt)) * want.abs())
+
+
+def test_attention_gradients_of_broadcast_keys():
+    q, do = rnd(1, 2, 70, 4, 32, grad=True), rnd(4, 2, 70, 4, 32)
+    k, v = rnd(2, 1, 70, 1, 32, grad=True), rnd(3, 1, 70, 1, 32, grad=True)
+    ke, ve = k.expand(2, 70, 4, 32), v.expand(2, 70, 4, 32)
+    g = torch.autograd.grad(A().window_attention(q, ke, ve, 9, 0, 1), (q, k, v), do)
+    ref = attn_ref(q, ke, ve, seen(70, 70, 9, 0, 1, 0, None, 2), 32 ** -0.5, F32, do)
+    within(g[0], *[t * 1.0 for t in (ref[1][0], ref[1][1] * 1.01 + 1e-30)])
+    for got, (r, e) in zip(g[1:], ref[2:]):
+        # (autograd adds the 2 x 4 copies in float32: 8 U of their magnitudes)
+        within(got, r.sum((0, 2), keepdim=True), (e * 1.01 + 8 * U * r.abs()).sum((0, 2), keepdim=True) + 1e-30)
 
 
 def test_attention_empty():
@@ -724,6 +751,33 @@ def test_side_streams():
     assert all(torch.equal(a, b) for a, b in zip(want + wr, got + gr))
 
 
+def test_beyond_32_bit_offsets():
+    """Tensors of more than 2^31 elements (4.6 GB each): the far end agrees with the same call on a slice of it.  The state
+    halves with every step (f = 0), so 64 steps ahead of the slice's last 64 leave 2^-64 of it; bfloat16 rounds both sides:
+    one step, 2 R, of the value, where they straddle a border."""
+    L, D = 2_200_000, 1024
+    x = torch.empty(1, L, D, dtype=BF, device=DEV)
+    x.view(-1, 1 << 10)[:] = rnd(1, 1 << 10, dt=BF)
+    x[0, -128:] = rnd(2, 128, D, dt=BF)
+    f = torch.zeros(1, 1, D, dtype=BF, device=DEV).expand(1, L, D)
+    y, _ = A().gated_recurrence(x, f)
+    want, _ = A().gated_recurrence(x[:, -128:], f[:, -128:])
+    a, b = y[:, -64:].double(), want[:, -64:].double()
+    assert float(((a - b).abs() - 2 * R(BF) * b.abs()).max()) <= 2.0 ** -60
+    q = x.view(1, L // 2, 16, 128)
+    k = q[:, :, :1]
+    o = A().window_attention(q, k, k, 20, 0)
+    # (against the formula on the slice: tiles cut the two calls' keys at different places, so bits may differ)
+    attn_check((o[:, -64:],), attn_ref(q[:, -64:], k[:, -128:], k[:, -128:], seen(64, 128, 20, 0, 0, 64, None, 1), 128 ** -0.5, BF))
+    del y, o, want
+    kc, vc = x.view(2, L // 2, 8, 128), torch.zeros(2, L // 2, 8, 128, dtype=BF, device=DEV)
+    vc[1, L // 2 - 5] = 3.0                                                   # one slot of 1.1 million, equal weights: 3 / M
+    out = A().window_attention_step(torch.zeros(2, 8, 128, dtype=BF, device=DEV), kc[:, 0].clone(), vc[:, 0].clone(), kc, vc,
+                                    torch.tensor([L, L], device=DEV), 1)
+    assert not out[0].any()
+    assert float((out[1].double() * (L // 2) - 3.0).abs().max()) <= 3.0 * 2 * R(BF)
+
+
 # --------------------------------------------------------------------------- #
 # refusals
 # --------------------------------------------------------------------------- #
@@ -754,12 +808,15 @@ def test_refusals():
         lambda: a.window_attention(q.double(), k.double(), k.double(), 3),
         lambda: a.window_attention(q, k.cpu(), k, 3),
         lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc[:, :5], pos),
-        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc, pos, 6),
-        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc, pos.int()),
-        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc, pos.cpu()),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc.clone(), pos, 6),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc.clone(), pos.int()),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc.clone(), pos.cpu()),
         lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc.bfloat16(), kc.bfloat16(), pos),
-        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc.transpose(2, 3).contiguous().transpose(2, 3), kc, pos),
-        lambda: a.window_cache_fill(k, k, kc, kc, 6), lambda: a.window_cache_fill(k, k[:, :2], kc, kc),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc.transpose(2, 3).contiguous().transpose(2, 3), kc.clone(), pos),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc, pos),
+        lambda: a.window_attention_step(q[:, 0], k[:, 0], k[:, 0], kc, kc[:1].clone().expand(2, 6, 2, 32), pos),
+        lambda: a.window_attention_step(q[:, 0].clone().requires_grad_(), k[:, 0], k[:, 0], kc, kc.clone(), pos),
+        lambda: a.window_cache_fill(k, k, kc, kc.clone(), 6), lambda: a.window_cache_fill(k, k[:, :2], kc, kc.clone()),
         lambda: a.rotary(q, k, tp.float(), freq), lambda: a.rotary(q, k, tp[:3], freq), lambda: a.rotary(q, k, tp, freq.float()),
         lambda: a.rotary(q, k[..., :16], tp, freq), lambda: a.rotary(q, k, tp, torch.ones(17, dtype=F64, device=DEV)),
         lambda: a.rotary(q, k, tp, freq.cpu()), lambda: a.rotary(q, k.bfloat16(), tp, freq),
