@@ -214,7 +214,9 @@ template <int N> __device__ __forceinline__ void unpark(const float* at, f32x16_
 }
 
 // What store_rows' rounding to bf16 leaves off.  D = sum(dO O) from O as rounded would carry 2^-9 of |dO| |O| into every
-// dP - D of the row, as much again as dS's own rounding where a row sees few keys; with the rest of O beside it that is 2^-17.
+// dP - D of the row, as much again as dS's own rounding where a row sees few keys; with the rest of O beside it that is 2^-17.  (Over n
+// keys O is sqrt(n) smaller: large windows do without, dtt_wattn_wants_rest: writing it took 9 of 75 us forward at 2 x 4096
+// rows, 16 / 4 heads of 128, window 512.)
 template <int DH>
 __device__ __forceinline__ void store_rest(bf16* row, const f32x16_t (&acc)[DH / 32], float mul, int lh) {
 #pragma unroll
@@ -366,7 +368,12 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     store_rows<T, DH>(out, o, live ? 1.f / l : 0.f, lh);
     if constexpr (sizeof(T) == 2)
         if (p.lo) store_rest<DH>((bf16*)p.lo + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH, o, live ? 1.f / l : 0.f, lh);
-    if (p.lse && lh == 0) p.lse[((int64_t)b * p.Hq + h) * p.Tq + i] = live ? m + log2f(l) : INFINITY;
+    if (p.lse && lh == 0) {
+        // (fp32: reference and log of the sum apart, their sum as one float would cost the weights 2^-24 of its size)
+        float* s = p.lse + ((int64_t)b * p.Hq + h) * p.Tq + i;
+        if constexpr (sizeof(T) == 4) s[0] = live ? m : INFINITY, s[(int64_t)p.B * p.Hq * p.Tq] = live ? log2f(l) : 0.f;
+        else s[0] = live ? m + log2f(l) : INFINITY;
+    }
 }
 
 // dq, and D = sum(dO O) per row for the dk / dv launch behind it
@@ -414,7 +421,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         dd = both_sum(dd);
     }
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
-    const float lse = p.lse[at];
+    const float lse = p.lse[at], lsum = sizeof(T) == 4 ? p.lse[at + (int64_t)p.B * p.Hq * p.Tq] : 0.f;
     if (live && lh == 0 && sp == 0) p.dd[at] = dd;
     f32x16_t dq[DH / 32];
 #pragma unroll
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
             if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse)) * (y[r] - dd);
+            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse) - lsum) * (y[r] - dd);
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     constexpr int PARK = SP > 1 ? KG * DH * 128 / (int)sizeof(T) : 0;
     static_assert(SP <= QN / 32, "a 32-row tile of a staged one for every wave that shares keys");
     __shared__ __align__(16) T mem[N > PARK ? N : PARK];
-    __shared__ __align__(16) float st[3][QN];     // per row: log of the sum, D, and 1 (0 where one key is seen: no gradient of weights)
+    __shared__ __align__(16) float st[sizeof(T) == 4 ? 4 : 3][QN];        // per row: log of the sum, D, and 1 (0 where one key is seen: no gradient of weights)
     T* qs = mem;
     T* gs = mem + TILE;
     T* vimg = mem + 2 * TILE;
@@ -553,7 +560,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     const float sc = p.scale * LOG2E;
     Stage<T, DH, QN, NT> sq(p.q_st), sg(p.g_st);
     const int per = r1 > r0 ? (r1 - r0 + QN - 1) / QN : 0, count = per * p.G;
-    float sl = 0.f, sd = 0.f, sw = 0.f;
+    float sl = 0.f, sd = 0.f, sw = 0.f, ss = 0.f;
     auto load = [&](int n) {
         const int h = hk * p.G + n / per, r = r0 + n % per * QN;
         sq.load((const T*)p.q + b * p.q_sb + h * p.q_sh, p.q_st, r, r1);
@@ -562,6 +569,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             const int i = r + threadIdx.x;
             const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + min(i, p.Tq - 1);
             const float lv = p.lse[at], dvv = p.dd[at];
+            if constexpr (sizeof(T) == 4) ss = p.lse[at + (int64_t)p.B * p.Hq * p.Tq];
             sl = i < r1 ? lv : INFINITY;
             sw = i < r1 && seen_keys(p, p.offset + i, klen) > 1 ? 1.f : 0.f;
             sd = sw != 0.f ? dvv : 0.f;
@@ -572,7 +580,10 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
         __syncthreads();
         sq.store(qs);
         sg.store(gs);
-        if (threadIdx.x < QN) st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd, st[2][threadIdx.x] = sw;
+        if (threadIdx.x < QN) {
+            st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd, st[2][threadIdx.x] = sw;
+            if constexpr (sizeof(T) == 4) st[3][threadIdx.x] = ss;
+        }
         __syncthreads();
         const int i0 = r0 + n % per * QN;
         if (n + 1 < count) load(n + 1);
@@ -607,7 +618,9 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * r4 + e;
-                    x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -(&ls.x)[e]));
+                    x[r] = fmaf(x[r], sc, -(&ls.x)[e]);
+                    if constexpr (sizeof(T) == 4) x[r] -= st[3][32 * s + 8 * r4 + 4 * lh + e];
+                    x[r] = __builtin_amdgcn_exp2f(x[r]);
                     y[r] = x[r] * fmaf(y[r], (&ws.x)[e], -(&ds.x)[e]);
                 }
             }
@@ -1040,6 +1053,12 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
 #undef FWD
     DTT_LAUNCH_CHECK();
     return 0;
+}
+
+extern "C" int dtt_wattn_wants_rest(const DttWattn* g) {
+    WaP p;
+    if (!g || wa_check(g, p, "dtt_wattn_wants_rest")) return 0;
+    return g->dtype == 1 && (split_rows(p) || split_keys(p) || fine(p));
 }
 
 extern "C" int64_t dtt_wattn_bwd_ws_bytes(const DttWattn* g) {

@@ -231,10 +231,10 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     out, lse, rest = torch.empty_like(q, memory_format=_ROWS), None, None
     g.out = out.data_ptr()
     if keep:
-        if q.dtype is BF16:
+        if lib().dtt_wattn_wants_rest(C.byref(g)):
             rest = torch.empty_like(out)
             g.out_rest = rest.data_ptr()
-        lse = torch.empty((B, Hq, Tq), dtype=F32, device=q.device)
+        lse = torch.empty((1 if q.dtype is BF16 else 2, B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
     check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
     return out, lse, rest, g
@@ -252,7 +252,7 @@ class WindowAttention(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, lengths, out, lse, rest = ctx.saved_tensors                  # (out, rest: alive; the struct has their addresses)
         do, g = _rows_attn(do), _again(ctx.call)
-        dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse)
+        dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
         g.g_sb, g.g_st, g.g_sh, _ = do.stride()
         lib_, ref = lib(), C.byref(g)
