@@ -489,21 +489,20 @@ int dtt_rotary(const DttRotary* g, void* stream);
 /* Windowed attention with first tokens that stay visible: the query at position p = offset + i sees key j where
  * j <= p + right and (j >= p - left or j < sinks); softmax(scale * q k^T) v over those; a row that sees none is zero.
  * lengths [B] (NULL: none): positions from lengths[b] on are padding: keys there are never read, rows there are zero and
- * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides (rows of one head DH to 2^22 elements apart, every row on 16 bytes); out, dq
- * [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
- * out_rest (bfloat16 only; may be NULL, in both calls alike): what out's rounding leaves off, of out's shape, so that the
- * backward's row sums do not carry it; dtt_wattn_wants_rest() is 1 where rows see so few keys that this shows.
- * lse [B][Hq][Tq], in float32 [2][B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call; dd [B][Hq][Tq]: scratch of
- * the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give equal bits. */
+ * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides (rows of one head DH to 2^22
+ * elements apart, every row on 16 bytes); out, dq [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of
+ * Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
+ * lse [B][Hq][Tq], in float32 [2][B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call;
+ * dd [B][Hq][Tq]: scratch of the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give
+ * equal bits. */
 typedef struct {
-    const void* q; const void* k; const void* v; void* out; void* out_rest; float* lse;
+    const void* q; const void* k; const void* v; void* out; float* lse;
     const void* dout; void* dq; void* dk; void* dv; float* dd;
     const int32_t* lengths; void* ws; int64_t ws_bytes;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
     int32_t B, Tq, Tk, Hq, Hk, DH, left, right, sinks, offset, dtype;
     float scale;
 } DttWattn;
-int dtt_wattn_wants_rest(const DttWattn* g);
 int dtt_wattn_fwd(const DttWattn* g, void* stream);
 int64_t dtt_wattn_bwd_ws_bytes(const DttWattn* g);
 int dtt_wattn_bwd(const DttWattn* g, void* stream);

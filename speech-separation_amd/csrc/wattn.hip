@@ -15,6 +15,7 @@
 // below.
 #include "common.h"
 #include "../../include/dtt_hip.h"
+#include <algorithm>
 
 namespace {
 constexpr int NTH = 256, BN = 64;                // threads (dk / dv: up to twice that); keys of a staged tile (forward, dq)
@@ -23,12 +24,12 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 struct WaP {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
-    void* out; void* lo; void* dq; void* dk; void* dv;
+    void* out; void* dq; void* dk; void* dv;
     float* lse; float* dd; float* part;
     const int* len;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
     int B, Tq, Tk, Hq, Hk, G, left, right, sinks, offset;
-    int nt, nchunk, chunk, npart, edge;          // tiles along the row axis; chunks of the rows from edge on (first tokens' gradients)
+    int nt, few, nchunk, chunk, npart, edge;          // tiles along the row axis; chunks of the rows from edge on (first tokens' gradients)
     float scale;
 };
 
@@ -213,26 +214,6 @@ template <int N> __device__ __forceinline__ void unpark(const float* at, f32x16_
         for (int r = 0; r < 16; ++r) a[c][r] = fmaf(at[(c * 16 + r) * 64 + lane], theirs, a[c][r] * mine);
 }
 
-// What store_rows' rounding to bf16 leaves off.  D = sum(dO O) from O as rounded would carry 2^-9 of |dO| |O| into every
-// dP - D of the row, as much again as dS's own rounding where a row sees few keys; with the rest of O beside it that is 2^-17.  (Over n
-// keys O is sqrt(n) smaller: large windows do without, dtt_wattn_wants_rest: writing it took 9 of 75 us forward at 2 x 4096
-// rows, 16 / 4 heads of 128, window 512.)
-template <int DH>
-__device__ __forceinline__ void store_rest(bf16* row, const f32x16_t (&acc)[DH / 32], float mul, int lh) {
-#pragma unroll
-    for (int ct = 0; ct < DH / 32; ++ct)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = acc[ct][4 * q + e] * mul;
-                v[e] = a - bf2f(f2bf(a));
-            }
-            *reinterpret_cast<uint2*>(row + 32 * ct + 8 * q + 4 * lh) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        }
-}
-
 // The key tiles (of N keys) that the query rows at positions p0 .. p1 see: [0, a) holds first tokens only, [b, c] the window.
 struct Tiles { int a, b, c; };
 template <int N> __device__ __forceinline__ Tiles key_tiles(const WaP& p, int p0, int p1, int klen) {
@@ -366,8 +347,6 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
         for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
     }
     store_rows<T, DH>(out, o, live ? 1.f / l : 0.f, lh);
-    if constexpr (sizeof(T) == 2)
-        if (p.lo) store_rest<DH>((bf16*)p.lo + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH, o, live ? 1.f / l : 0.f, lh);
     if (p.lse && lh == 0) {
         // (fp32: reference and log of the sum apart, their sum as one float would cost the weights 2^-24 of its size)
         float* s = p.lse + ((int64_t)b * p.Hq + h) * p.Tq + i;
@@ -384,6 +363,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
     constexpr bool FINE = sizeof(T) == 2 && SP == 2;           // dS in two bf16 pieces, see fine()
     __shared__ __align__(16) T img[2 * BN * I::LD];
+    __shared__ float half[SP > 1 ? NTH / 64 : 1][32];
     static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, rg = SP > 1 ? wave % RG : wave, sp = SP > 1 ? wave / RG : 0;
     int id = xcd_order(blockIdx.x, gridDim.x);
@@ -404,25 +384,20 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
         gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
     }
-    // D by the matrix cores, as the diagonal of O dO^T
+    // D = sum(dO O) by the matrix cores, as the diagonal of O dO^T; or, where rows see few keys, by a walk of its own over the
+    // keys as sum(P dP), see fine()
+    const bool walk = SP == 2 && p.few;
     float dd = 0.f;
-    {
+    if (!walk) {
         f32x16_t t = zero_acc();
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) MM<T>::mma(MM<T>::ldfrag(oo + 16 * c + 8 * lh), gf[c], t);
-        if constexpr (sizeof(T) == 2)
-            if (p.lo) {
-                const T* lo = (const T*)p.lo + (oo - (const T*)p.o) + 8 * lh;
-#pragma unroll
-                for (int c = 0; c < DH / 16; ++c) MM<T>::mma(MM<T>::ldfrag(lo + 16 * c), gf[c], t);
-            }
 #pragma unroll
         for (int r = 0; r < 16; ++r) dd += acc_row(r, lh) == lr ? t[r] : 0.f;
         dd = both_sum(dd);
     }
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
     const float lse = p.lse[at], lsum = sizeof(T) == 4 ? p.lse[at + (int64_t)p.B * p.Hq * p.Tq] : 0.f;
-    if (live && lh == 0 && sp == 0) p.dd[at] = dd;
     f32x16_t dq[DH / 32];
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
@@ -439,13 +414,20 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         sv.load(v, p.v_st, r0, klen);
     };
     if (count > 0) load(0);
-    for (int n = 0; n < count; ++n) {
+    for (int w = walk ? -count : 0; w < count; ++w) {                       // w < 0: the walk for D
+        const int n = w < 0 ? w + count : w;
+        if (walk && w == 0) {                                               // both waves' halves of D
+            dd = both_sum(dd);
+            half[wave][lr] = dd;
+            __syncthreads();
+            dd = half[rg][lr] + half[(rg + RG) % (NTH / 64)][lr];
+        }
         __syncthreads();
         sk.store(ks);
         sv.store(vs);
         __syncthreads();
         const int j0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
-        if (n + 1 < count) load(n + 1);
+        if (w + 1 < count) load(n + 1 < count ? n + 1 : 0);
 #pragma unroll
         for (int k = 0; k < BN / 32 / SP; ++k) {
             const int s = k * SP + sp, js = j0 + 32 * s;
@@ -458,6 +440,11 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
             }
             const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
             if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
+            if (w < 0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dd = fmaf(__builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse) - lsum), y[r], dd);
+                continue;
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse) - lsum) * (y[r] - dd);
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
@@ -471,6 +458,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
                 }
         }
     }
+    if (live && lh == 0 && sp == 0) p.dd[at] = dd;
     if constexpr (SP > 1) {
         float* mem = reinterpret_cast<float*>(img) + rg * DH * 32;
         __syncthreads();
@@ -986,7 +974,7 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
     p = WaP{};
     p.q = g->q; p.k = g->k; p.v = g->v; p.o = g->out; p.out = g->out; p.dout = g->dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
-    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths; p.lo = g->dtype ? g->out_rest : nullptr;
+    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
     // (strides of axes of one element do not count)
     const bool b = g->B > 1, tq = g->Tq > 1, tk = g->Tk > 1, hq = g->Hq > 1, hk = g->Hk > 1;
     p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : g->DH; p.q_sh = hq ? g->q_sh : 0;
@@ -1018,10 +1006,12 @@ int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk
 // the other way: forward 69 -> 85 us at 2 x 4096 rows, 16 / 4 heads.  512 workgroups are two a CU.
 bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
 bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
-// Rows of few keys: the rounding of dS to bf16 (2^-9 of each) does not average out over two or three keys, and dq and dk come
-// out 1.5 to 1.6 times as far from the exact ones as their own rounding is; over 20 keys and more it is 1.4.  The kernels for few rows
-// carry what the rounding leaves off as a second operand (a third more matrix instructions); small windows take them too.
-bool fine(const WaP& p) { return (int64_t)p.left + p.right + p.sinks < 24; }
+// Rows of few keys.  The rounding of dS to bf16 (2^-9 of each) does not average out over two or three keys, and D = sum(dO O)
+// does not cancel against dP as sum(P dP) does (bf16: O's own rounding; fp32: two sums in different orders, which shows
+// where one key has nearly all the weight): dq and dk came out 1.5 to 1.8 times (fp32: 6 times) as far from the exact ones
+// as plain arithmetic in 32 bits.  The kernels for few rows carry what the rounding of dS leaves off as a second operand,
+// and where no row can see more than 32 keys they form D by a walk of its own, one or two tiles long; small windows take them too.
+bool fine(const WaP& p) { return std::min<int64_t>((int64_t)p.left + p.right + 1 + p.sinks, p.Tk) <= 32; }
 
 #define WA_DH(FN, T)                                                              \
     do {                                                                          \
@@ -1037,7 +1027,7 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     DTT_CHECK(g, "dtt_wattn_fwd: null argument");
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_fwd")) return rc;
-    DTT_CHECK(g->out && aligned16(g->out) && aligned16(g->out_rest), "dtt_wattn_fwd: null or unaligned output");
+    DTT_CHECK(g->out && aligned16(g->out), "dtt_wattn_fwd: null or unaligned output");
     const bool split = split_rows(p);
     const int bm = split ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
@@ -1055,12 +1045,6 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     return 0;
 }
 
-extern "C" int dtt_wattn_wants_rest(const DttWattn* g) {
-    WaP p;
-    if (!g || wa_check(g, p, "dtt_wattn_wants_rest")) return 0;
-    return g->dtype == 1 && (split_rows(p) || split_keys(p) || fine(p));
-}
-
 extern "C" int64_t dtt_wattn_bwd_ws_bytes(const DttWattn* g) {
     WaP p;
     if (!g || wa_check(g, p, "dtt_wattn_bwd_ws_bytes")) return 0;
@@ -1073,14 +1057,15 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_bwd")) return rc;
     DTT_CHECK(g->out && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
-    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->out_rest) && aligned16(g->dout) && aligned16(g->dq) &&
+    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
               aligned16(g->dk) && aligned16(g->dv), "dtt_wattn_bwd: rows must start on 16 bytes");
     far_chunks(p);
     const int64_t need = part_bytes(p, g->DH);
     DTT_CHECK(need == 0 || (g->ws && aligned16(g->ws) && g->ws_bytes >= need), "dtt_wattn_bwd: workspace of %lld bytes, %lld given",
               (long long)need, (long long)g->ws_bytes);
     p.part = (float*)g->ws;
-    const bool split = split_rows(p) || fine(p), splitk = split_keys(p) || fine(p);
+    p.few = fine(p);
+    const bool split = split_rows(p) || p.few, splitk = split_keys(p) || p.few;
     const int bm = split ? 64 : 128, km = splitk ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
     WaP pk = p;

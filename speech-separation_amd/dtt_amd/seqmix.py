@@ -228,29 +228,26 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
     if lengths is not None:
         g.lengths = lengths.data_ptr()
-    out, lse, rest = torch.empty_like(q, memory_format=_ROWS), None, None
+    out, lse = torch.empty_like(q, memory_format=_ROWS), None
     g.out = out.data_ptr()
     if keep:
-        if lib().dtt_wattn_wants_rest(C.byref(g)):
-            rest = torch.empty_like(out)
-            g.out_rest = rest.data_ptr()
         lse = torch.empty((1 if q.dtype is BF16 else 2, B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
     check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
-    return out, lse, rest, g
+    return out, lse, g
 
 
 class WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, cfg):
-        out, lse, rest, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
-        ctx.save_for_backward(q, k, v, lengths, out, lse, rest)
+        out, lse, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
+        ctx.save_for_backward(q, k, v, lengths, out, lse)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, lengths, out, lse, rest = ctx.saved_tensors                  # (out, rest: alive; the struct has their addresses)
+        q, k, v, lengths, out, lse = ctx.saved_tensors                        # (out: alive; the struct has its address)
         do, g = _rows_attn(do), _again(ctx.call)
         dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
