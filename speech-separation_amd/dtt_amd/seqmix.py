@@ -79,6 +79,17 @@ def _lengths(name, lengths, batch, first):
     return (lengths if lengths.dtype is I32 else lengths.clamp(-1, (1 << 31) - 1).to(I32)).contiguous()
 
 
+def _first_order(backward):
+    """backward() without a derivative of its own: once_differentiable where a graph of the backward pass is recorded (which
+    then refuses second derivatives), the bare function where none is."""
+    refuses = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return refuses(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
+
+
 def _workspace(g, need, dev):
     """Scratch for one call; the caller keeps the tensor until the call is enqueued (the caching allocator orders reuse)."""
     if need <= 0:
@@ -134,8 +145,7 @@ class GatedRecurrence(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y, last
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dlast):
         x, f, h0, lengths, states = ctx.saved_tensors
         g = _again(ctx.call)
@@ -143,7 +153,7 @@ class GatedRecurrence(torch.autograd.Function):
         if dlast is not None:
             dlast = dlast.contiguous()
             g.dlast = dlast.data_ptr()
-        dx, df, dh0 = x.new_empty(x.shape), x.new_empty(x.shape), None
+        dx, df, dh0 = torch.empty_like(x, memory_format=_ROWS), torch.empty_like(x, memory_format=_ROWS), None
         if h0 is not None and ctx.needs_input_grad[2]:
             dh0 = torch.empty_like(h0)
             g.dh0 = dh0.data_ptr()
@@ -244,12 +254,12 @@ class WindowAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, lengths, out, lse)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, do):
         q, k, v, lengths, out, lse = ctx.saved_tensors                        # (out: alive; the struct has its address)
         do, g = _rows_attn(do), _again(ctx.call)
-        dq, dk, dv, dd = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), torch.empty_like(lse[0])
+        dq, dk, dv = (torch.empty_like(t, memory_format=_ROWS) for t in (q, k, v))
+        dd = torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
         g.g_sb, g.g_st, g.g_sh, _ = do.stride()
         lib_, ref = lib(), C.byref(g)
@@ -432,8 +442,7 @@ class Rotary(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return _rotate(q, k, _again(g))
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dq, dk):
         ctx.saved_tensors                                                     # (raises if positions or freq were overwritten)
         g = _again(ctx.call)

@@ -778,6 +778,18 @@ def test_beyond_32_bit_offsets():
     assert float((out[1].double() * (L // 2) - 3.0).abs().max()) <= 3.0 * 2 * R(BF)
 
 
+def test_second_derivatives_are_refused():
+    """A gradient taken with create_graph is right; differentiating it again raises instead of giving zeros."""
+    q, x, f = rnd(1, 1, 20, 2, 32, grad=True), rnd(2, 1, 20, 8, grad=True), rnd(3, 1, 20, 8, grad=True)
+    freq, pos = A().rotary_frequencies(32, device=DEV), torch.arange(20, device=DEV)
+    for fn, leaf in ((lambda: A().window_attention(q, q, q, 5), q), (lambda: A().gated_recurrence(x, f)[0], x),
+                     (lambda: A().rotary(q, q, pos, freq)[0], q)):
+        g, = torch.autograd.grad(fn().square().sum(), leaf, create_graph=True)
+        assert torch.equal(g, torch.autograd.grad(fn().square().sum(), leaf)[0])
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), leaf)
+
+
 # --------------------------------------------------------------------------- #
 # refusals
 # --------------------------------------------------------------------------- #
