@@ -995,7 +995,7 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
 void far_chunks(WaP& p) {
     const int64_t edge = (int64_t)MAX_SINKS + p.left - p.offset;          // behind the window of every tile with first tokens
     p.edge = p.sinks == 0 || edge >= p.Tq ? p.Tq : edge > 0 ? (int)edge : 0;
-    p.chunk = 128;
+    p.chunk = std::max(128, (p.Tq - p.edge + 511) / 512 / 64 * 64 + 64);  // (512 chunks at most, or the partials outgrow the gradients)
     p.nchunk = p.sinks ? (p.Tq - p.edge + p.chunk - 1) / p.chunk : 0;
     p.npart = 1 + 2 * p.nchunk;
 }

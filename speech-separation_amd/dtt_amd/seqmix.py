@@ -100,7 +100,8 @@ def _workspace(g, need, dev):
 
 
 def _again(g):
-    """A copy of a forward call's struct: backward calls of one graph may run at the same time."""
+    """A copy of a forward call's struct (backward calls of one graph may run at the same time), for its sizes: the addresses
+    are those of the forward call, and hooks on saved tensors (checkpoints, offloading) hand back others."""
     return type(g).from_buffer_copy(g)
 
 
@@ -112,19 +113,21 @@ def _rec_strides(t):
     return s[:3] if len(s) == 4 else (s[0], 0, s[1])
 
 
+def _rec_inputs(g, x, f, h0, lengths):
+    g.x, g.f = x.data_ptr(), f.data_ptr()
+    g.x_so, g.x_si, g.x_sl = _rec_strides(x)
+    g.f_so, g.f_si, g.f_sl = _rec_strides(f)
+    g.lengths = None if lengths is None else lengths.data_ptr()
+    g.h0 = None if h0 is None else h0.data_ptr()
+
+
 def _rec_forward(x, f, h0, reverse, lengths, keep):
     shape = x.shape
     L, D = shape[-2:]
     N = math.prod(shape[:-2])
     g = DttRecurrence(N=N, NI=shape[1] if len(shape) == 4 else 1, L=L, D=D, reverse=1 if reverse else 0,
                       dtype=1 if x.dtype is BF16 else 0)
-    g.x, g.f = x.data_ptr(), f.data_ptr()
-    g.x_so, g.x_si, g.x_sl = _rec_strides(x)
-    g.f_so, g.f_si, g.f_sl = _rec_strides(f)
-    if lengths is not None:
-        g.lengths = lengths.data_ptr()
-    if h0 is not None:
-        g.h0 = h0.data_ptr()
+    _rec_inputs(g, x, f, h0, lengths)
     y = torch.empty_like(x, memory_format=_ROWS)
     last = torch.empty(shape[:-2] + shape[-1:], dtype=F32, device=x.device)
     g.y, g.last = y.data_ptr(), last.data_ptr()
@@ -148,7 +151,9 @@ class GatedRecurrence(torch.autograd.Function):
     @_first_order
     def backward(ctx, dy, dlast):
         x, f, h0, lengths, states = ctx.saved_tensors
-        g = _again(ctx.call)
+        g, x, f = _again(ctx.call), _inner(x), _inner(f)
+        _rec_inputs(g, x, f, h0, lengths)
+        g.states = states.data_ptr()
         dy = x.new_zeros(x.shape[-1]).expand(x.shape) if dy is None else _inner(dy)
         if dlast is not None:
             dlast = dlast.contiguous()
@@ -228,16 +233,19 @@ def gated_recurrence_step(x, f, state):
 # --------------------------------------------------------------------------- #
 # windowed attention
 # --------------------------------------------------------------------------- #
-def _attn_forward(q, k, v, lengths, cfg, keep):
-    B, Tq, Hq, dh = q.shape
-    g = DttWattn(B=B, Tq=Tq, Tk=k.shape[1], Hq=Hq, Hk=k.shape[2], DH=dh, left=cfg[0], right=cfg[1], sinks=cfg[2], offset=cfg[3],
-                 dtype=1 if q.dtype is BF16 else 0, scale=cfg[4])
+def _attn_inputs(g, q, k, v, lengths):
     g.q, g.k, g.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     g.q_sb, g.q_st, g.q_sh, _ = q.stride()
     g.k_sb, g.k_st, g.k_sh, _ = k.stride()
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
-    if lengths is not None:
-        g.lengths = lengths.data_ptr()
+    g.lengths = None if lengths is None else lengths.data_ptr()
+
+
+def _attn_forward(q, k, v, lengths, cfg, keep):
+    B, Tq, Hq, dh = q.shape
+    g = DttWattn(B=B, Tq=Tq, Tk=k.shape[1], Hq=Hq, Hk=k.shape[2], DH=dh, left=cfg[0], right=cfg[1], sinks=cfg[2], offset=cfg[3],
+                 dtype=1 if q.dtype is BF16 else 0, scale=cfg[4])
+    _attn_inputs(g, q, k, v, lengths)
     out, lse = torch.empty_like(q, memory_format=_ROWS), None
     g.out = out.data_ptr()
     if keep:
@@ -256,8 +264,10 @@ class WindowAttention(torch.autograd.Function):
 
     @_first_order
     def backward(ctx, do):
-        q, k, v, lengths, out, lse = ctx.saved_tensors                        # (out: alive; the struct has its address)
-        do, g = _rows_attn(do), _again(ctx.call)
+        q, k, v, lengths, out, lse = ctx.saved_tensors
+        q, k, v, do, g = _rows_attn(q), _rows_attn(k), _rows_attn(v), _rows_attn(do), _again(ctx.call)
+        _attn_inputs(g, q, k, v, lengths)
+        g.out, g.lse = out.data_ptr(), lse.data_ptr()
         dq, dk, dv = (torch.empty_like(t, memory_format=_ROWS) for t in (q, k, v))
         dd = torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
@@ -434,6 +444,12 @@ def _rotate(q, k, g):
     return qo, ko
 
 
+def _rot_inputs(g, positions, freq):
+    g.positions, g.freq, g.p_st = positions.data_ptr(), freq.data_ptr(), positions.stride(-1)
+    if positions.dim() == 2:
+        g.p_sb = positions.stride(0)
+
+
 class Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, freq, g):
@@ -444,9 +460,10 @@ class Rotary(torch.autograd.Function):
 
     @_first_order
     def backward(ctx, dq, dk):
-        ctx.saved_tensors                                                     # (raises if positions or freq were overwritten)
+        positions, freq = ctx.saved_tensors
         g = _again(ctx.call)
         g.back = 1
+        _rot_inputs(g, positions, freq)
         if dq is None:
             return (None, None if dk is None else _rotate(_inner(dk), None, g)[0], None, None, None)
         return _rotate(_inner(dq), None if dk is None else _inner(dk), g) + (None, None, None)
@@ -486,9 +503,7 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
             return rotary(q, k, positions, freq, interleaved, amplitude)
     g = DttRotary(B=B, T=T, dh=dh, r=2 * freq.shape[0], interleaved=1 if interleaved else 0, pos64=1 if positions.dtype is I64 else 0,
                   dtype=1 if q.dtype is BF16 else 0, amplitude=amplitude)
-    g.positions, g.freq, g.p_st = positions.data_ptr(), freq.data_ptr(), positions.stride(-1)
-    if pd == 2:
-        g.p_sb = positions.stride(0)
+    _rot_inputs(g, positions, freq)
     q = _inner(q)
     if k is None:
         return Rotary.apply(q, None, positions, freq, g)[0] if torch.is_grad_enabled() and q.requires_grad else _rotate(q, None, g)[0]

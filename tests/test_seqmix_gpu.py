@@ -778,6 +778,33 @@ def test_beyond_32_bit_offsets():
     assert float((out[1].double() * (L // 2) - 3.0).abs().max()) <= 3.0 * 2 * R(BF)
 
 
+@pytest.mark.parametrize("how", ["checkpoint", "offload"])
+def test_hooks_on_saved_tensors(how):
+    """Recomputed (checkpoint) and moved (offload) saved tensors give the gradients of kept ones, bit by bit."""
+    from torch.utils.checkpoint import checkpoint
+    w = rnd(1, 64, 3 * 64, std=0.2, grad=True)
+    x = rnd(2, 2, 150, 64, grad=True)
+    freq, pos = A().rotary_frequencies(32, device=DEV), torch.arange(150, device=DEV)
+    lens = torch.tensor([150, 90], device=DEV, dtype=torch.int32)
+
+    def block(x):
+        q, k, v = (t.unflatten(-1, (2, 32)) for t in (x @ w).chunk(3, -1))
+        q, k = A().rotary(q, k, pos, freq)
+        o = A().window_attention(q, k, v, 20, 0, 2, lengths=lens).flatten(2)
+        return A().gated_recurrence(o, o * 2, lengths=lens)[0]
+
+    want = torch.autograd.grad(block(x).square().sum(), (x, w))
+    if how == "checkpoint":
+        got = torch.autograd.grad(checkpoint(block, x, use_reentrant=False).square().sum(), (x, w))
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            y = block(x).square().sum()
+        junk = [torch.full((2, 150, 192), math.nan, device=DEV) for _ in range(20)]      # (what a stale address would read)
+        got = torch.autograd.grad(y, (x, w))
+        del junk
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_second_derivatives_are_refused():
     """A gradient taken with create_graph is right; differentiating it again raises instead of giving zeros."""
     q, x, f = rnd(1, 1, 20, 2, 32, grad=True), rnd(2, 1, 20, 8, grad=True), rnd(3, 1, 20, 8, grad=True)
