@@ -1110,10 +1110,11 @@ int ws_check(const DttWattnStep* g, WsP& p, const char* what) {
               (g->dtype ? 8 : 4) == 0 && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(g->kc) && aligned16(g->vc),
               "%s: rows must start on 16 bytes", what);
     p.B = g->B; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk; p.ngrp = (p.G + 31) / 32; p.S = g->S; p.W = g->W; p.scale = g->scale;
-    // splits of the slots: while fewer than four workgroups a CU, ranges of 512 slots at least (four tiles a wave)
+    // splits of the slots: where there is less than a workgroup a CU, ranges of 512 slots at least (four tiles a wave).  One a
+    // CU reads at the full rate already: 64 streams over 4016 slots, 16 / 4 heads of 128, 93 us, with four splits 99 + 6
     const int M = g->S + g->W;
     const int64_t rows = (int64_t)p.B * p.Hk * p.ngrp;
-    int64_t ns = 1024 / rows, most = (M + 511) / 512;
+    int64_t ns = 256 / rows, most = (M + 511) / 512;
     ns = ns < 1 ? 1 : ns > most ? most : ns;
     p.per = (int)(((M + ns - 1) / ns + 127) / 128 * 128);
     p.nsplit = (M + p.per - 1) / p.per;
