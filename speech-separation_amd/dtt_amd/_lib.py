@@ -34,6 +34,15 @@ def lib():
         _lib.dtt_multi_pack_nchunks.restype = C.c_int64
         for name in ("dtt_recurrence_ws_bytes", "dtt_recurrence_states", "dtt_wattn_bwd_ws_bytes", "dtt_wattn_step_ws_bytes"):
             getattr(_lib, name).restype = C.c_int64
+        # the calls of seqmix.py: typed, so that addresses and strides go in as plain ints (a c_void_p object each costs as
+        # much as the check of an argument)
+        vp, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+        for name in ("dtt_recurrence_fwd", "dtt_recurrence_bwd", "dtt_rotary", "dtt_wattn_fwd", "dtt_wattn_bwd", "dtt_wattn_step"):
+            getattr(_lib, name).argtypes = [vp, vp]
+        for name in ("dtt_recurrence_ws_bytes", "dtt_recurrence_states", "dtt_wattn_bwd_ws_bytes", "dtt_wattn_step_ws_bytes"):
+            getattr(_lib, name).argtypes = [vp]
+        _lib.dtt_recurrence_step.argtypes = [vp, vp, vp, vp, i32, i32, i64, i64, i32, vp]
+        _lib.dtt_wattn_cache_fill.argtypes = [vp, vp, i32, vp]
     return _lib
 
 

@@ -18,14 +18,20 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import lib, check, stream_ptr, dtype_code, DttError, DttRecurrence, DttRotary, DttWattn, DttWattnStep
+from ._lib import lib, check, dtype_code, DttError, DttRecurrence, DttRotary, DttWattn, DttWattnStep
 
 # The single-frame forms and short training steps are bound by what the host spends on a call: arguments are checked with
 # plain comparisons (messages are formatted on failure alone), structs are filled once and kept for the backward call.
 
 F32, BF16, F64, I32, I64 = torch.float32, torch.bfloat16, torch.float64, torch.int32, torch.int64
-_device = torch._C._cuda_getDevice
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _ROWS = torch.contiguous_format
+_addr = C.addressof
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 # --------------------------------------------------------------------------- #
@@ -36,10 +42,12 @@ def _fail(name, what):
 
 
 def _on_gpu(name, t):
+    """The index of t's GPU; refuses other devices and types."""
     if not t.is_cuda:
         _fail(name, "dtt_amd ops need CUDA(HIP) tensors; there is no CPU path")
     if t.dtype is not F32 and t.dtype is not BF16:
         dtype_code(t.dtype)
+    return t.get_device()
 
 
 def _beside(name, t, what, other):
@@ -131,12 +139,12 @@ def _rec_forward(x, f, h0, reverse, lengths, keep):
     y = torch.empty_like(x, memory_format=_ROWS)
     last = torch.empty(shape[:-2] + shape[-1:], dtype=F32, device=x.device)
     g.y, g.last = y.data_ptr(), last.data_ptr()
-    lib_, ref, states = lib(), C.byref(g), None
+    lib_, ref, states = lib(), _addr(g), None
     if keep:
         states = torch.empty(lib_.dtt_recurrence_states(ref), dtype=F32, device=x.device)
         g.states = states.data_ptr()
     ws = _workspace(g, lib_.dtt_recurrence_ws_bytes(ref), x.device)  # noqa: F841 (alive until the call returns)
-    check(lib_.dtt_recurrence_fwd(ref, stream_ptr()), "dtt_recurrence_fwd")
+    check(lib_.dtt_recurrence_fwd(ref, _stream(x.get_device())), "dtt_recurrence_fwd")
     return y, last, states, g
 
 
@@ -164,9 +172,9 @@ class GatedRecurrence(torch.autograd.Function):
             g.dh0 = dh0.data_ptr()
         g.dy, g.dx, g.df = dy.data_ptr(), dx.data_ptr(), df.data_ptr()
         g.g_so, g.g_si, g.g_sl = _rec_strides(dy)
-        lib_, ref = lib(), C.byref(g)
+        lib_, ref = lib(), _addr(g)
         ws = _workspace(g, lib_.dtt_recurrence_ws_bytes(ref), x.device)  # noqa: F841
-        check(lib_.dtt_recurrence_bwd(ref, stream_ptr()), "dtt_recurrence_bwd")
+        check(lib_.dtt_recurrence_bwd(ref, _stream(x.get_device())), "dtt_recurrence_bwd")
         return dx, df, dh0, None, None
 
 
@@ -181,10 +189,11 @@ def gated_recurrence(x, f, h0=None, reverse=False, lengths=None):
     name = "gated_recurrence"
     if not torch.is_tensor(x) or not torch.is_tensor(f) or x.dim() not in (3, 4) or x.shape != f.shape:
         _fail(name, "x and f must have one shape, [B, L, D] or [B, N, L, D]")
-    _on_gpu(name, x)
+    dev = _on_gpu(name, x)
     if x.dtype is not f.dtype:
         _fail(name, f"x is {x.dtype}, f is {f.dtype}")
-    _beside(name, x, "f", f)
+    if f.get_device() != dev:
+        _beside(name, x, "f", f)
     batch = x.shape[:-2]
     if h0 is not None:
         if h0.dtype is not F32 or h0.shape != batch + x.shape[-1:]:
@@ -194,8 +203,8 @@ def gated_recurrence(x, f, h0=None, reverse=False, lengths=None):
         lengths = _lengths(name, lengths, batch, x)
     if x.numel() == 0:
         return x * f, (h0.clone() if h0 is not None else torch.zeros(batch + x.shape[-1:], dtype=F32, device=x.device))
-    if x.get_device() != _device():
-        with torch.cuda.device(x.device):
+    if dev != _device():
+        with torch.cuda.device(dev):
             return gated_recurrence(x, f, h0, reverse, lengths)
     x, f = _inner(x), _inner(f)
     if h0 is not None:
@@ -209,24 +218,30 @@ def gated_recurrence_step(x, f, state):
     """One step of gated_recurrence for every item: x, f [N, D], state float32 [N, D] (contiguous), replaced by the new
     state; returns it in x's dtype.  No gradients."""
     name = "gated_recurrence_step"
-    if x.dim() != 2 or x.shape != f.shape or x.shape != state.shape:
+    shape = x.shape
+    if len(shape) != 2 or f.shape != shape or state.shape != shape:
         _fail(name, "x, f and state must have one shape [N, D]")
-    _on_gpu(name, x)
-    if x.dtype is not f.dtype or state.dtype is not F32 or not state.is_contiguous():
+    dev, dt = _on_gpu(name, x), x.dtype
+    if f.dtype is not dt or state.dtype is not F32 or not state.is_contiguous():
         _fail(name, "x and f must have one dtype, state must be float32 and contiguous")
-    if f.device != x.device or state.device != x.device:
+    if f.get_device() != dev or state.get_device() != dev:
         _fail(name, "x, f and state must be on one device")
     if torch.is_grad_enabled() and (x.requires_grad or f.requires_grad or state.requires_grad):
         _fail(name, "no gradient: call it under torch.no_grad()")
-    if x.get_device() != _device():
-        with torch.cuda.device(x.device):
+    if dev != _device():
+        with torch.cuda.device(dev):
             return gated_recurrence_step(x, f, state)
-    N, D = x.shape
-    x, f, y = _inner(x), _inner(f), torch.empty_like(x, memory_format=_ROWS)
+    N, D = shape
+    (xs, xe), (fs, fe) = x.stride(), f.stride()
+    if xe != 1 or fe != 1:
+        x, f = _inner(x), _inner(f)
+        xs, fs = x.stride(0), f.stride(0)
+    y = torch.empty_like(x, memory_format=_ROWS)
     if N * D:
-        check(lib().dtt_recurrence_step(C.c_void_p(x.data_ptr()), C.c_void_p(f.data_ptr()), C.c_void_p(state.data_ptr()),
-                                        C.c_void_p(y.data_ptr()), N, D, C.c_int64(x.stride(0)), C.c_int64(f.stride(0)),
-                                        1 if x.dtype is BF16 else 0, stream_ptr()), "dtt_recurrence_step")
+        rc = lib().dtt_recurrence_step(x.data_ptr(), f.data_ptr(), state.data_ptr(), y.data_ptr(), N, D, xs, fs,
+                                       1 if dt is BF16 else 0, _stream(dev))
+        if rc:
+            check(rc, "dtt_recurrence_step")
     return y
 
 
@@ -251,7 +266,7 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     if keep:
         lse = torch.empty((1 if q.dtype is BF16 else 2, B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
-    check(lib().dtt_wattn_fwd(C.byref(g), stream_ptr()), "dtt_wattn_fwd")
+    check(lib().dtt_wattn_fwd(_addr(g), _stream(q.get_device())), "dtt_wattn_fwd")
     return out, lse, g
 
 
@@ -272,27 +287,32 @@ class WindowAttention(torch.autograd.Function):
         dd = torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()
         g.g_sb, g.g_st, g.g_sh, _ = do.stride()
-        lib_, ref = lib(), C.byref(g)
+        lib_, ref = lib(), _addr(g)
         ws = _workspace(g, lib_.dtt_wattn_bwd_ws_bytes(ref), q.device)  # noqa: F841 (alive until the call returns)
-        check(lib_.dtt_wattn_bwd(ref, stream_ptr()), "dtt_wattn_bwd")
+        check(lib_.dtt_wattn_bwd(ref, _stream(q.get_device())), "dtt_wattn_bwd")
         return dq, dk, dv, None, None
 
 
 def _heads_check(name, q, k, v, dims):
-    if not (torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v)) or q.dim() != dims or k.dim() != dims:
-        _fail(name, f"q, k and v must be tensors of {dims} axes")
-    _on_gpu(name, q)
+    """The index of the tensors' GPU."""
+    if not (torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v)):
+        _fail(name, "q, k and v must be tensors")
     qs, ks = q.shape, k.shape
+    if len(qs) != dims or len(ks) != dims:
+        _fail(name, f"q, k and v must have {dims} axes")
+    dev, dt = _on_gpu(name, q), q.dtype
     if ks != v.shape or ks[0] != qs[0] or ks[-1] != qs[-1]:
         _fail(name, f"shapes {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)} do not fit")
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
+    if k.dtype is not dt or v.dtype is not dt:
         _fail(name, "q, k and v must have one dtype")
-    if k.device != q.device or v.device != q.device:
+    if k.get_device() != dev or v.get_device() != dev:
         _fail(name, f"q, k and v are on {q.device}, {k.device} and {v.device}")
-    if qs[-2] == 0 or ks[-2] == 0 or qs[-2] % ks[-2]:
-        _fail(name, f"{qs[-2]} query heads over {ks[-2]} key heads")
+    hq, hk = qs[-2], ks[-2]
+    if hq == 0 or hk == 0 or hq % hk:
+        _fail(name, f"{hq} query heads over {hk} key heads")
     if qs[-1] not in (32, 64, 96, 128):
         _fail(name, f"head width {qs[-1]} (32, 64, 96 or 128)")
+    return dev
 
 
 _BIG = 1 << 28
@@ -308,7 +328,7 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
     are never read, rows there are zero and take no part in any gradient.  A non-finite key or value inside lengths may
     reach rows of the same 32 positions that do not see it.  Differentiable in q, k and v."""
     name = "window_attention"
-    _heads_check(name, q, k, v, 4)
+    dev = _heads_check(name, q, k, v, 4)
     Tq, Tk = q.shape[1], k.shape[1]
     offset = Tk - Tq if offset is None else int(offset)
     left, right, sinks = int(left), int(right), int(sinks)
@@ -321,8 +341,8 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if q.numel() == 0 or Tk == 0:
         return q * 0.0 + k.sum() * 0.0 + v.sum() * 0.0 if grad else torch.zeros_like(q)
-    if q.get_device() != _device():
-        with torch.cuda.device(q.device):
+    if dev != _device():
+        with torch.cuda.device(dev):
             return window_attention(q, k, v, left, right, sinks, lengths, offset, scale)
     cfg = (min(left, _BIG), min(right, _BIG), sinks, offset, q.shape[-1] ** -0.5 if scale is None else float(scale))
     q, k, v = _rows_attn(q), _rows_attn(k), _rows_attn(v)
@@ -336,7 +356,7 @@ def _step_args(name, k, v, k_cache, v_cache, sinks, scale):
         _fail(name, f"caches must be [B, sinks + window, Hk, dh], got {tuple(cs)} and {tuple(v_cache.shape)}")
     if k_cache.dtype is not k.dtype or v_cache.dtype is not k.dtype:
         _fail(name, "caches must have the dtype of k")
-    if k_cache.device != k.device or v_cache.device != k.device:
+    if k_cache.get_device() != k.get_device() or v_cache.get_device() != k.get_device():
         _fail(name, "caches must be on the device of k")
     if not 0 <= sinks < cs[1]:
         _fail(name, f"sinks={sinks} of {cs[1]} slots (at least one for the window)")
@@ -359,14 +379,15 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, sinks=0, scale=N
     q [B, Hq, dh] to every slot filled so far: what window_attention(left=window - 1, sinks=sinks) gives for that row.
     An item with a negative position is idle: its cache stays as it is and its row is zero.  No gradients."""
     name = "window_attention_step"
-    _heads_check(name, q, k, v, 3)
+    dev = _heads_check(name, q, k, v, 3)
     if positions.dtype is not I64 or positions.dim() != 1 or positions.shape[0] != q.shape[0] or not positions.is_contiguous():
         _fail(name, "positions must be a contiguous int64 tensor [B]")
-    _beside(name, q, "positions", positions)
+    if positions.get_device() != dev:
+        _beside(name, q, "positions", positions)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         _fail(name, "no gradient: call it under torch.no_grad()")
-    if q.get_device() != _device():
-        with torch.cuda.device(q.device):
+    if dev != _device():
+        with torch.cuda.device(dev):
             return window_attention_step(q, k, v, k_cache, v_cache, positions, sinks, scale)
     out = torch.empty_like(q, memory_format=_ROWS)
     if q.shape[0] == 0:
@@ -378,9 +399,9 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, sinks=0, scale=N
     g.q_sb, g.q_sh, _ = q.stride()
     g.k_sb, g.k_sh, _ = k.stride()
     g.v_sb, g.v_sh, _ = v.stride()
-    lib_, ref = lib(), C.byref(g)
+    lib_, ref = lib(), _addr(g)
     ws = _workspace(g, lib_.dtt_wattn_step_ws_bytes(ref), q.device)  # noqa: F841 (alive until the call returns)
-    check(lib_.dtt_wattn_step(ref, stream_ptr()), "dtt_wattn_step")
+    check(lib_.dtt_wattn_step(ref, _stream(dev)), "dtt_wattn_step")
     return out
 
 
@@ -403,8 +424,8 @@ def window_cache_fill(k, v, k_cache, v_cache, sinks=0, lengths=None):
     g.k, g.v = k.data_ptr(), v.data_ptr()
     g.k_sb, g.k_st, g.k_sh, _ = k.stride()
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
-    check(lib().dtt_wattn_cache_fill(C.byref(g), C.c_void_p(None if lengths is None else lengths.data_ptr()), k.shape[1],
-                                     stream_ptr()), "dtt_wattn_cache_fill")
+    check(lib().dtt_wattn_cache_fill(_addr(g), None if lengths is None else lengths.data_ptr(), k.shape[1],
+                                     _stream(k.get_device())), "dtt_wattn_cache_fill")
 
 
 # --------------------------------------------------------------------------- #
@@ -440,7 +461,7 @@ def _rotate(q, k, g):
         g.k_sb, g.k_st, g.k_sh, _ = k.stride()
     else:
         g.Hk = 0
-    check(lib().dtt_rotary(C.byref(g), stream_ptr()), "dtt_rotary")
+    check(lib().dtt_rotary(_addr(g), _stream(q.get_device())), "dtt_rotary")
     return qo, ko
 
 
@@ -479,26 +500,26 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
     name = "rotary"
     if not torch.is_tensor(q) or q.dim() != 4:
         _fail(name, "q must be [B, T, H, dh]")
-    _on_gpu(name, q)
+    dev = _on_gpu(name, q)
     B, T, _, dh = q.shape
-    dev = q.device
     if k is not None:
         ks = k.shape
         if len(ks) != 4 or ks[0] != B or ks[1] != T or ks[3] != dh or k.dtype is not q.dtype:
             _fail(name, f"q {tuple(q.shape)} {q.dtype} and k {tuple(ks)} {k.dtype} must agree in all but heads")
-        _beside(name, q, "k", k)
+        if k.get_device() != dev:
+            _beside(name, q, "k", k)
     pd = positions.dim()
     if positions.dtype not in (I64, I32) or positions.shape != ((T,) if pd == 1 else (B, T)):
         _fail(name, f"positions must be int32 or int64 [T] or [B, T], got {positions.dtype} {tuple(positions.shape)}")
     if freq.dtype is not F64 or freq.dim() != 1 or not freq.is_contiguous() or not 0 < 2 * freq.shape[0] <= min(dh, 4096):
         _fail(name, "freq must be a contiguous float64 vector of 1 to dh / 2 elements (2048 at most)")
-    if positions.device != dev or freq.device != dev:
-        _fail(name, f"positions and freq must be on {dev}")
+    if positions.get_device() != dev or freq.get_device() != dev:
+        _fail(name, f"positions and freq must be on {q.device}")
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         if q.numel() or (k is not None and k.numel()):
             _fail(name, "q and k must both have heads")
         return q.clone() if k is None else (q.clone(), k.clone())
-    if q.get_device() != _device():
+    if dev != _device():
         with torch.cuda.device(dev):
             return rotary(q, k, positions, freq, interleaved, amplitude)
     g = DttRotary(B=B, T=T, dh=dh, r=2 * freq.shape[0], interleaved=1 if interleaved else 0, pos64=1 if positions.dtype is I64 else 0,
