@@ -9,6 +9,8 @@
 // steps and combine by shuffles and one LDS exchange, and the tile is finished from the same registers -- x and f are
 // read once.  States are fp32 throughout.  The forward pass keeps the state at every tile's start; the backward
 // pass recomputes the tile's states from it (in fp32: the rounded y would not do for h_{t-1} - x_t) instead of reading y.
+// Measured, bf16: 1040 x 47 x 1024 75 us forward (4.0 TB/s), 104 backward (4.8 TB/s); 2 x 15001 x 1024, cut into
+// segments whose maps a launch of its own finds first: 41 + 35 and 25 + 58 us.
 #include "common.h"
 #include "../../include/dtt_hip.h"
 
