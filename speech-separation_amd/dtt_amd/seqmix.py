@@ -55,6 +55,12 @@ def _beside(name, t, what, other):
         _fail(name, f"{what} is on {other.device}, the other tensors on {t.device}")
 
 
+def _sizes(name, t):
+    """Refuses axes (and, of the axes before the last two, products) that 32 bits do not hold; t is known to be large."""
+    if max(t.shape) >> 31 or math.prod(t.shape[:-2]) >> 31:
+        _fail(name, f"shape {tuple(t.shape)}: sizes must be below 2^31")
+
+
 def _inner(t):
     """`t` with a contiguous innermost axis, a copy if it has not."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.clone(memory_format=torch.contiguous_format)
@@ -206,6 +212,8 @@ def gated_recurrence(x, f, h0=None, reverse=False, lengths=None):
     if dev != _device():
         with torch.cuda.device(dev):
             return gated_recurrence(x, f, h0, reverse, lengths)
+    if x.numel() >> 31:
+        _sizes(name, x)
     x, f = _inner(x), _inner(f)
     if h0 is not None:
         h0 = h0.contiguous()
@@ -232,6 +240,8 @@ def gated_recurrence_step(x, f, state):
         with torch.cuda.device(dev):
             return gated_recurrence_step(x, f, state)
     N, D = shape
+    if N * D >> 31:
+        _sizes(name, x)
     (xs, xe), (fs, fe) = x.stride(), f.stride()
     if xe != 1 or fe != 1:
         x, f = _inner(x), _inner(f)
@@ -312,6 +322,8 @@ def _heads_check(name, q, k, v, dims):
         _fail(name, f"{hq} query heads over {hk} key heads")
     if qs[-1] not in (32, 64, 96, 128):
         _fail(name, f"head width {qs[-1]} (32, 64, 96 or 128)")
+    if q.numel() >> 31:
+        _sizes(name, q)
     return dev
 
 
@@ -340,7 +352,7 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
         lengths = _lengths(name, lengths, q.shape[:1], q)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if q.numel() == 0 or Tk == 0:
-        return q * 0.0 + k.sum() * 0.0 + v.sum() * 0.0 if grad else torch.zeros_like(q)
+        return torch.zeros_like(q) + sum(t[..., :0].sum() for t in (q, k, v)) if grad else torch.zeros_like(q)
     if dev != _device():
         with torch.cuda.device(dev):
             return window_attention(q, k, v, left, right, sinks, lengths, offset, scale)
@@ -358,8 +370,8 @@ def _step_args(name, k, v, k_cache, v_cache, sinks, scale):
         _fail(name, "caches must have the dtype of k")
     if k_cache.get_device() != k.get_device() or v_cache.get_device() != k.get_device():
         _fail(name, "caches must be on the device of k")
-    if not 0 <= sinks < cs[1]:
-        _fail(name, f"sinks={sinks} of {cs[1]} slots (at least one for the window)")
+    if not 0 <= sinks < cs[1] or cs[1] >> 30:
+        _fail(name, f"sinks={sinks} of {cs[1]} slots (at least one for the window, less than 2^30)")
     g = DttWattnStep(B=cs[0], Hq=cs[2], Hk=cs[2], DH=cs[3], S=sinks, W=cs[1] - sinks, dtype=1 if k.dtype is BF16 else 0, scale=scale)
     g.kc_sb, g.kc_st, g.kc_sh, ke = k_cache.stride()
     g.vc_sb, g.vc_st, g.vc_sh, ve = v_cache.stride()
@@ -519,6 +531,10 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
         if q.numel() or (k is not None and k.numel()):
             _fail(name, "q and k must both have heads")
         return q.clone() if k is None else (q.clone(), k.clone())
+    if q.numel() >> 31:
+        _sizes(name, q)
+    if k is not None and k.numel() >> 31:
+        _sizes(name, k)
     if dev != _device():
         with torch.cuda.device(dev):
             return rotary(q, k, positions, freq, interleaved, amplitude)

@@ -865,3 +865,29 @@ def test_refusals():
         with pytest.raises(DttError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_sizes_beyond_32_bits():
+    """Refused before anything is allocated (such a size would be cut to its low 32 bits on its way to C)."""
+    n = (1 << 32) + 1
+    x, t = torch.zeros(1, 1, 1, device=DEV).expand(n, 1, 1), torch.zeros(1, 1, 1, 32, device=DEV).expand(n, 1, 1, 32)
+    freq = A().rotary_frequencies(32, device=DEV)
+    for call in (lambda: A().gated_recurrence(x, x),
+                 lambda: A().gated_recurrence(x.view(1, n, 1, 1), x.view(1, n, 1, 1)),
+                 lambda: A().window_attention(t, t, t, 1),
+                 lambda: A().rotary(t, None, torch.zeros(1, dtype=torch.int64, device=DEV), freq),
+                 lambda: A().rotary(t[:1], t[:1].expand(1, 1, n, 32), torch.zeros(1, dtype=torch.int64, device=DEV), freq)):
+        with pytest.raises(A().DttError):
+            call()
+
+
+@pytest.mark.parametrize("tq,tk", [(3, 0), (0, 3)])
+def test_attention_without_rows_or_keys(tq, tk):
+    """No key: rows of zeros whatever q holds; zero gradients both ways."""
+    q = torch.full((2, tq, 2, 32), float("nan"), device=DEV, requires_grad=True)
+    k, v = (torch.full((2, tk, 1, 32), float("nan"), device=DEV, requires_grad=True) for _ in range(2))
+    out = A().window_attention(q, k, v, 4, sinks=1, offset=0)
+    assert out.shape == q.shape and bool((out == 0).all())
+    out.sum().backward()
+    for t in (q, k, v):
+        assert t.grad.shape == t.shape and bool((t.grad == 0).all())
