@@ -8,8 +8,10 @@
 // so that the softmax statistics are per-lane scalars and one exchange with lane ^ 32, and the tile's accumulator
 // registers, packed to the compute type, already are the B operand of O^T += V^T P^T: register r of a 16-key chunk holds key
 // (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and V^T's fragments are read from LDS in that order of keys.
-// P and dS are rounded to the compute type there (bf16: half a step, up to 2^-8 relative each, at the size of the outputs' own
-// rounding); statistics, accumulators, D = sum(dO O) and sinks' partial sums stay fp32.
+// In bf16 the weights P enter their products as two operands, P rounded and what that left off (2^-16 of a weight in all): with
+// the first alone (2^-8) the outputs were 1.4 times as far from the exact ones as their own rounding puts them, whatever the
+// window (forward 2.22e-3 against 1.63e-3 relative, dv 2.33e-3 against 1.66e-3).  dS is rounded to bf16 once but where fine()
+// applies; statistics, accumulators, D = sum(dO O) and sinks' partial sums stay fp32.
 //
 // Bound: the matrix cores (4 DH flops per visible pair forward, 10 DH backward) for windows beyond a few hundred keys, HBM
 // below.  Measured, bf16, 2 x 4096 rows, 16 / 4 heads of 128, window 512 + 4 first tokens (114 GF, 92 us at the rate of a
@@ -90,11 +92,16 @@ template <typename T> __device__ __forceinline__ typename MM<T>::Frag acc_frag(c
         return f;
     }
 }
-// what acc_frag's rounding leaves off registers 8 c .. 8 c + 7, as a fragment (bf16)
-__device__ __forceinline__ s16x8_t rest_frag(const f32x16_t& s, int c) {
+// what the rounding of acc_frag left off registers 8 c .. 8 c + 7 (bf16), as a second operand fragment: the two pieces hold a
+// value to 2^-16 of it
+__device__ __forceinline__ s16x8_t rest_frag(const f32x16_t& s, int c, const s16x8_t& first) {
+    const uint4 u = __builtin_bit_cast(uint4, first);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = s[8 * c + e] - bf2f(f2bf(s[8 * c + e]));
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t w = (&u.x)[e >> 1];
+        v[e] = s[8 * c + e] - __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+    }
     return __builtin_bit_cast(s16x8_t, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
 }
 __device__ __forceinline__ f32x16_t zero_acc() {
@@ -320,8 +327,14 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag pf = acc_frag<T>(x[n], c);
+                    Frag pr;
+                    if constexpr (sizeof(T) == 2) pr = rest_frag(x[n], c, pf);
 #pragma unroll
-                    for (int ct = 0; ct < DH / 32; ++ct) MM<T>::mma(tr_frag_of<T, DH>(vs, 32 * (sub + n) + 16 * c, 32 * ct), pf, o[ct]);
+                    for (int ct = 0; ct < DH / 32; ++ct) {
+                        const Frag vt = tr_frag_of<T, DH>(vs, 32 * (sub + n) + 16 * c, 32 * ct);
+                        MM<T>::mma(vt, pf, o[ct]);
+                        if constexpr (sizeof(T) == 2) MM<T>::mma(vt, pr, o[ct]);
+                    }
                 }
         }
     }
@@ -456,7 +469,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
                 for (int ct = 0; ct < DH / 32; ++ct) {
                     const Frag kt = tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct);
                     MM<T>::mma(kt, pf[c], dq[ct]);
-                    if constexpr (FINE) MM<T>::mma(kt, rest_frag(x, c), dq[ct]);
+                    if constexpr (FINE) MM<T>::mma(kt, rest_frag(x, c, pf[c]), dq[ct]);
                 }
         }
     }
@@ -543,7 +556,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             if constexpr (KL) st16<T>(kimg + I::at(r, pc), ld16_pred<T>(k + (int64_t)jv * p.k_st + pc * I::EPP, k, jv < klen));
         }
     }
-    const int vr = (far ? 0 : kg * 32) + lr;      // this lane's row there
+    const int vrow = (far ? 0 : kg * 32) + lr;    // this lane's row there
     f32x16_t dk[DH / 32], dv[DH / 32];
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dk[c] = zero_acc(), dv[c] = zero_acc();
@@ -583,6 +596,9 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             if (far && (it || wave >= QN / 32)) continue;
             const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
+            int vr = vrow;
+            // (the addresses of K's and V's fragments are formed anew for every tile: kept in registers they were spilled)
+            if constexpr (KL) asm volatile("" : "+v"(vr));
             f32x16_t x = zero_acc(), y = zero_acc();
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
@@ -614,17 +630,34 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
                     y[r] = x[r] * fmaf(y[r], (&ws.x)[e], -(&ds.x)[e]);
                 }
             }
-            const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
-            const Frag df[2] = {acc_frag<T>(y, 0), acc_frag<T>(y, 1)};
-#pragma unroll
-            for (int ct = 0; ct < DH / 32; ++ct)
+            if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    MM<T>::mma(tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct), pf[c], dv[ct]);
-                    const Frag qt = tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct);
-                    MM<T>::mma(qt, df[c], dk[ct]);
-                    if constexpr (FINE) MM<T>::mma(qt, rest_frag(y, c), dk[ct]);
+                    const Frag pf = acc_frag<T>(x, c), pr = rest_frag(x, c, pf);
+                    const Frag df = acc_frag<T>(y, c);
+                    Frag dr;
+                    if constexpr (FINE) dr = rest_frag(y, c, df);
+#pragma unroll
+                    for (int ct = 0; ct < DH / 32; ++ct) {
+                        const Frag gt = tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct);
+                        MM<T>::mma(gt, pf, dv[ct]);
+                        MM<T>::mma(gt, pr, dv[ct]);
+                        const Frag qt = tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct);
+                        MM<T>::mma(qt, df, dk[ct]);
+                        if constexpr (FINE) MM<T>::mma(qt, dr, dk[ct]);
+                    }
                 }
+            } else {
+                const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
+                const Frag df[2] = {acc_frag<T>(y, 0), acc_frag<T>(y, 1)};
+#pragma unroll
+                for (int ct = 0; ct < DH / 32; ++ct)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        MM<T>::mma(tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct), pf[c], dv[ct]);
+                        MM<T>::mma(tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct), df[c], dk[ct]);
+                    }
+            }
         }
     }
     if (SP > 1 && !far) {
@@ -764,7 +797,11 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_step_kernel
 #pragma unroll
         for (int ct = 0; ct < DH / 32; ++ct)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) MM<T>::mma(tr_frag_of<T, DH>(img, 16 * c, 32 * ct), pf[c], o[ct]);
+            for (int c = 0; c < 2; ++c) {
+                const Frag vt = tr_frag_of<T, DH>(img, 16 * c, 32 * ct);
+                MM<T>::mma(vt, pf[c], o[ct]);
+                if constexpr (sizeof(T) == 2) MM<T>::mma(vt, rest_frag(x, c, pf[c]), o[ct]);
+            }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // and its reads ahead of the next writes
     }
     l = both_sum(l);

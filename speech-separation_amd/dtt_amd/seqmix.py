@@ -337,8 +337,9 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
     q [B, Tq, Hq, dh], k, v [B, Tk, Hk, dh] of one dtype, Hq a multiple of Hk (query head h reads key head
     h // (Hq // Hk)), dh 32, 64, 96 or 128; ``sinks`` <= 128.  ``offset`` defaults to Tk - Tq (the queries are the last
     Tq positions), ``scale`` (positive) to dh ** -0.5.  ``lengths`` [B]: positions from lengths on are padding -- keys there
-    are never read, rows there are zero and take no part in any gradient.  A non-finite key or value inside lengths may
-    reach rows of the same 32 positions that do not see it.  Differentiable in q, k and v."""
+    are never read, rows there are zero and take no part in any gradient.  A non-finite key or value inside lengths gives
+    NaN, also in rows of the same 32 positions that do not see it.  bfloat16: weights enter their products with 16 bits,
+    sums are float32, results are rounded once.  Differentiable in q, k and v."""
     name = "window_attention"
     dev = _heads_check(name, q, k, v, 4)
     Tq, Tk = q.shape[1], k.shape[1]

@@ -1,0 +1,77 @@
+"""The token mixers' bfloat16 results are the exact ones rounded once, up to what 32-bit sums and weights of 16 bits leave: every
+element within half a step of its own binade and a bound far below that, counted in float64 beside the reference.
+
+U = 2^-24.  A score is a sum of dh products in float32, (dh + 8) U of their magnitudes; a weight is an exponential of
+a score less the log of the row's sum, both below 16 here: 48 U in all for the roundings of the two, of the exponential and of the
+sum, n U for the sum over n keys.  A weight (and dS) enters its product in two bfloat16 pieces, 2^-16 of it."""
+import math
+
+import pytest
+import torch
+from test_seqmix_gpu import A, BF, DEV, F64, rnd, seen
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+PIECES = 2.0 ** -16
+
+
+def rounded_once(got, ref, err, what):
+    """got is a bfloat16 neighbour of a value within err of ref: off by err and half a step of the binade it lies in."""
+    top = (ref.abs() + err).clamp(min=2.0 ** -120)
+    half = torch.exp2(torch.floor(torch.log2(top)) - 8)
+    over = (got.detach().double() - ref).abs() - half - err
+    assert got.dtype == BF and torch.isfinite(got).all() and float(over.max()) <= 0.0, (what, float(over.max()))
+
+
+def bounds(q, k, v, see, scale, do):
+    """o, dv [B, T, H, dh] in float64 with the errors their kernels may have ahead of the final rounding."""
+    B, Tq, Hq, dh = q.shape
+    n, Hk = k.shape[1:3]
+    G = Hq // Hk
+    qd, kd, vd, dd = (t.detach().double().transpose(1, 2) for t in (q, k, v, do))
+    qd, dd = qd.reshape(B, Hk, G, Tq, dh), dd.reshape(B, Hk, G, Tq, dh)
+    kd, vd, sm = kd[:, :, None], vd[:, :, None], see[:, None, None]
+    s = qd @ kd.transpose(-1, -2) * scale
+    assert float(s[sm.expand_as(s)].abs().max()) * math.log2(math.e) + math.log2(n) < 16
+    P = torch.softmax(torch.where(sm, s, -math.inf), -1).nan_to_num(0.0)
+    es = torch.where(sm, (dh + 8) * U * scale * (qd.abs() @ kd.abs().transpose(-1, -2)), 0.0)
+    w = 2 * es.amax(-1, keepdim=True) + 48 * U + n * U
+    back = lambda t, H, T: t.reshape(B, H, T, dh).transpose(1, 2)  # noqa: E731
+    o, eo = P @ vd, (w + PIECES + n * U) * (P @ vd.abs())
+    dv, edv = (P.transpose(-1, -2) @ dd).sum(2), ((P * (w + PIECES + Tq * G * U)).transpose(-1, -2) @ dd.abs()).sum(2)
+    return {"o": (back(o, Hq, Tq), back(eo, Hq, Tq)), "dv": (back(dv, Hk, n), back(edv, Hk, n))}
+
+
+def case(B, T, Hq, Hk, dh):
+    """Scores of half a standard deviation: their own errors stay far below a weight's rounding to bfloat16."""
+    q, k = (rnd(s, B, T, h, dh, dt=BF, std=0.5, grad=True) for s, h in ((1, Hq), (2, Hk)))
+    return q, k, rnd(3, B, T, Hk, dh, dt=BF, grad=True), rnd(4, B, T, Hq, dh, dt=BF)
+
+
+CASES = [  # B, T, Hq, Hk, left, right, sinks: few row tiles and many
+    (2, 200, 2, 1, 20, 0, 0), (2, 200, 4, 2, 150, 4, 3), (64, 140, 4, 4, 20, 12, 0), (32, 180, 8, 4, 33, 0, 4),
+]
+
+
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,T,Hq,Hk,left,right,sinks", CASES)
+def test_attention_and_values_gradient_are_rounded_once(dh, B, T, Hq, Hk, left, right, sinks):
+    q, k, v, do = case(B, T, Hq, Hk, dh)
+    o = A().window_attention(q, k, v, left, right, sinks)
+    dv, = torch.autograd.grad(o, v, do)
+    want = bounds(q, k, v, seen(T, T, left, right, sinks, 0, None, B), dh ** -0.5, do)
+    rounded_once(o, *want["o"], "o")
+    rounded_once(dv, *want["dv"], "dv")
+
+
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,Hq,Hk,window,sinks", [(40, 8, 2, 60, 2), (3, 4, 4, 900, 0)])
+def test_a_frame_is_rounded_once(dh, B, Hq, Hk, window, sinks):
+    M = window + sinks
+    q, k, v = rnd(1, B, Hq, dh, dt=BF, std=0.5), rnd(2, B, Hk, dh, dt=BF, std=0.5), rnd(3, B, Hk, dh, dt=BF)
+    kc, vc = rnd(4, B, M, Hk, dh, dt=BF, std=0.5), rnd(5, B, M, Hk, dh, dt=BF)
+    pos = torch.randint(0, 2 * M, (B,), generator=torch.Generator().manual_seed(7)).to(DEV)
+    out = A().window_attention_step(q, k, v, kc, vc, pos, sinks)
+    see = (torch.arange(M, device=DEV)[None] <= pos[:, None])[:, None]
+    ref, err = bounds(q[:, None], kc, vc, see, dh ** -0.5, torch.zeros_like(q)[:, None])["o"]
+    rounded_once(out, ref[:, 0], err[:, 0], "frame")
