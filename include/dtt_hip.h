@@ -493,10 +493,11 @@ int dtt_rotary(const DttRotary* g, void* stream);
  * elements apart, every row on 16 bytes); out, dq [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of
  * Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
  * lse [B][Hq][Tq], in float32 [2][B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call;
+ * rest [B][Tq][Hq][DH] (bfloat16 only; forward: may be NULL): what the rounding of out left off, for the backward call;
  * dd [B][Hq][Tq]: scratch of the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give
  * equal bits. */
 typedef struct {
-    const void* q; const void* k; const void* v; void* out; float* lse;
+    const void* q; const void* k; const void* v; void* out; void* rest; float* lse;
     const void* dout; void* dq; void* dk; void* dv; float* dd;
     const int32_t* lengths; void* ws; int64_t ws_bytes;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;

@@ -8,10 +8,10 @@
 // so that the softmax statistics are per-lane scalars and one exchange with lane ^ 32, and the tile's accumulator
 // registers, packed to the compute type, already are the B operand of O^T += V^T P^T: register r of a 16-key chunk holds key
 // (r & 3) + 8 (r >> 2) + 4 (lane >> 5), and V^T's fragments are read from LDS in that order of keys.
-// In bf16 the weights P enter their products as two operands, P rounded and what that left off (2^-16 of a weight in all): with
-// the first alone (2^-8) the outputs were 1.4 times as far from the exact ones as their own rounding puts them, whatever the
-// window (forward 2.22e-3 against 1.63e-3 relative, dv 2.33e-3 against 1.66e-3).  dS is rounded to bf16 once but where fine()
-// applies; statistics, accumulators, D = sum(dO O) and sinks' partial sums stay fp32.
+// In bf16 the weights P and dS enter their products as two operands, the rounded value and what that left off (2^-16 of it in
+// all): with the first alone (2^-8) results were 1.4 times as far from the exact ones as their own rounding puts them,
+// whatever the window (o 2.22e-3 against 1.63e-3 relative, dv 2.33e-3 and dq 2.42e-3 against 1.66e-3).  Statistics,
+// accumulators, D = sum(dO O) and first tokens' partial sums stay fp32.
 //
 // Bound: the matrix cores (4 DH flops per visible pair forward, 10 DH backward) for windows beyond a few hundred keys, HBM
 // below.  Measured, bf16, 2 x 4096 rows, 16 / 4 heads of 128, window 512 + 4 first tokens (114 GF, 92 us at the rate of a
@@ -28,7 +28,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 struct WaP {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
-    void* out; void* dq; void* dk; void* dv;
+    void* out; void* rest; void* dq; void* dk; void* dv;
     float* lse; float* dd; float* part;
     const int* len;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
@@ -153,17 +153,26 @@ __device__ __forceinline__ int xcd_order(int id, int n) {
     return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
 }
 
-// 4 consecutive channels per register group of an O^T-shaped accumulator: row pointer + 32 ct + 8 q + 4 lh
+// 4 consecutive channels per register group of an O^T-shaped accumulator: row pointer + 32 ct + 8 q + 4 lh.  rest (bf16, may be
+// null): the same row's place for what the rounding left off
 template <typename T, int DH>
-__device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32], float mul, int lh) {
+__device__ __forceinline__ void store_rows(T* row, const f32x16_t (&acc)[DH / 32], float mul, int lh, T* rest = nullptr) {
 #pragma unroll
     for (int ct = 0; ct < DH / 32; ++ct)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             T* o = row + 32 * ct + 8 * q + 4 * lh;
             const float a = acc[ct][4 * q] * mul, b = acc[ct][4 * q + 1] * mul, c = acc[ct][4 * q + 2] * mul, d = acc[ct][4 * q + 3] * mul;
-            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
-            else *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+            if constexpr (sizeof(T) == 2) {
+                const uint32_t u = pack_bf16x2(a, b), w = pack_bf16x2(c, d);
+                *reinterpret_cast<uint2*>(o) = make_uint2(u, w);
+                if (rest)
+                    *reinterpret_cast<uint2*>(rest + (o - row)) =
+                        make_uint2(pack_bf16x2(a - __uint_as_float(u << 16), b - __uint_as_float(u & 0xffff0000u)),
+                                   pack_bf16x2(c - __uint_as_float(w << 16), d - __uint_as_float(w & 0xffff0000u)));
+            } else {
+                *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+            }
         }
 }
 
@@ -356,12 +365,12 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     }
     if (i >= p.Tq) return;
     const bool live = pos < qlen && l != 0.f;         // (l is at least 1 where anything is visible; NaN passes)
-    T* out = (T*)p.out + (((int64_t)b * p.Tq + i) * p.Hq + h) * DH;
+    const int64_t row = (((int64_t)b * p.Tq + i) * p.Hq + h) * DH;
     if (!live) {
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) o[c] = zero_acc();
     }
-    store_rows<T, DH>(out, o, live ? 1.f / l : 0.f, lh);
+    store_rows<T, DH>((T*)p.out + row, o, live ? 1.f / l : 0.f, lh, p.rest ? (T*)p.rest + row : nullptr);
     if (p.lse && lh == 0) {
         // (fp32: reference and log of the sum apart, their sum as one float would cost the weights 2^-24 of its size)
         float* s = p.lse + ((int64_t)b * p.Hq + h) * p.Tq + i;
@@ -376,7 +385,6 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
-    constexpr bool FINE = sizeof(T) == 2 && SP == 2;           // dS in two bf16 pieces, see fine()
     __shared__ __align__(16) T img[2 * BN * I::LD];
     __shared__ float half[SP > 1 ? NTH / 64 : 1][32];
     static_assert(RG * SP * 64 == NTH && (SP == 1 || (SP == 2 && RG * DH * 128 <= (int)sizeof(img))), "");
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
     const bool live = i < p.Tq && pos < qlen;
     const T* q = (const T*)p.q + b * p.q_sb + (int64_t)ic * p.q_st + h * p.q_sh;
     const T* go = (const T*)p.dout + b * p.g_sb + (int64_t)ic * p.g_st + h * p.g_sh;
-    const T* oo = (const T*)p.o + (((int64_t)b * p.Tq + ic) * p.Hq + h) * DH;
+    const int64_t row = (((int64_t)b * p.Tq + ic) * p.Hq + h) * DH;
     const T* kp = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
     Frag qf[DH / 16], gf[DH / 16];
@@ -399,14 +407,17 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
         gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
     }
-    // D = sum(dO O) by the matrix cores, as the diagonal of O dO^T; or, where rows see few keys, by a walk of its own over the
-    // keys as sum(P dP), see fine()
+    // D = sum(dO O) by the matrix cores, as the diagonal of O dO^T (bf16: of O and what its rounding left off: D cancels against
+    // dP, which is not rounded to 8 bits); or, where rows see few keys, by a walk of its own over the keys as sum(P dP), see fine()
     const bool walk = SP == 2 && p.few;
     float dd = 0.f;
     if (!walk) {
         f32x16_t t = zero_acc();
 #pragma unroll
-        for (int c = 0; c < DH / 16; ++c) MM<T>::mma(MM<T>::ldfrag(oo + 16 * c + 8 * lh), gf[c], t);
+        for (int c = 0; c < DH / 16; ++c) {
+            MM<T>::mma(MM<T>::ldfrag((const T*)p.o + row + 16 * c + 8 * lh), gf[c], t);
+            if constexpr (sizeof(T) == 2) MM<T>::mma(MM<T>::ldfrag((const T*)p.rest + row + 16 * c + 8 * lh), gf[c], t);
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) dd += acc_row(r, lh) == lr ? t[r] : 0.f;
         dd = both_sum(dd);
@@ -469,7 +480,7 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
                 for (int ct = 0; ct < DH / 32; ++ct) {
                     const Frag kt = tr_frag_of<T, DH>(ks, 32 * s + 16 * c, 32 * ct);
                     MM<T>::mma(kt, pf[c], dq[ct]);
-                    if constexpr (FINE) MM<T>::mma(kt, rest_frag(x, c, pf[c]), dq[ct]);
+                    if constexpr (sizeof(T) == 2) MM<T>::mma(kt, rest_frag(x, c, pf[c]), dq[ct]);
                 }
         }
     }
@@ -503,7 +514,6 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     // V's fragments (and K's) are read from LDS where with both sums, both tiles and the next rows on their way they would
     // exceed the registers of two waves a SIMD (fp32: of one)
     constexpr int KM = 32 * KG, NT = KG * SP * 64;
-    constexpr bool FINE = sizeof(T) == 2 && KG == 2;           // dS in two bf16 pieces, see fine()
     constexpr bool VL = DH >= 96, KL = DH == 128 && sizeof(T) == 2 && KG * SP == 8;
     constexpr int TILE = QN * I::LD, OWN = KM * I::LD, N = 2 * TILE + (VL ? OWN : 0) + (KL ? OWN : 0);
     constexpr int PARK = SP > 1 ? KG * DH * 128 / (int)sizeof(T) : 0;
@@ -634,9 +644,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag pf = acc_frag<T>(x, c), pr = rest_frag(x, c, pf);
-                    const Frag df = acc_frag<T>(y, c);
-                    Frag dr;
-                    if constexpr (FINE) dr = rest_frag(y, c, df);
+                    const Frag df = acc_frag<T>(y, c), dr = rest_frag(y, c, df);
 #pragma unroll
                     for (int ct = 0; ct < DH / 32; ++ct) {
                         const Frag gt = tr_frag_of<T, DH>(gs, 32 * s + 16 * c, 32 * ct);
@@ -644,7 +652,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
                         MM<T>::mma(gt, pr, dv[ct]);
                         const Frag qt = tr_frag_of<T, DH>(qs, 32 * s + 16 * c, 32 * ct);
                         MM<T>::mma(qt, df, dk[ct]);
-                        if constexpr (FINE) MM<T>::mma(qt, dr, dk[ct]);
+                        MM<T>::mma(qt, dr, dk[ct]);
                     }
                 }
             } else {
@@ -1013,7 +1021,7 @@ int wa_check(const DttWattn* g, WaP& p, const char* what) {
     DTT_CHECK(g->q && g->k && g->v, "%s: null buffer", what);
     p = WaP{};
     p.q = g->q; p.k = g->k; p.v = g->v; p.o = g->out; p.out = g->out; p.dout = g->dout; p.dq = g->dq; p.dk = g->dk; p.dv = g->dv;
-    p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
+    p.rest = g->dtype ? g->rest : nullptr; p.lse = g->lse; p.dd = g->dd; p.len = g->lengths;
     // (strides of axes of one element do not count)
     const bool b = g->B > 1, tq = g->Tq > 1, tk = g->Tk > 1, hq = g->Hq > 1, hk = g->Hk > 1;
     p.q_sb = b ? g->q_sb : 0; p.q_st = tq ? g->q_st : g->DH; p.q_sh = hq ? g->q_sh : 0;
@@ -1045,11 +1053,9 @@ int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk
 // the other way: forward 69 -> 85 us at 2 x 4096 rows, 16 / 4 heads.  512 workgroups are two a CU.
 bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
 bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
-// Rows of few keys.  The rounding of dS to bf16 (up to 2^-8 of each) does not average out over two or three keys, and D = sum(dO O)
-// does not cancel against dP as sum(P dP) does (bf16: O's own rounding; fp32: two sums in different orders, which shows
-// where one key has nearly all the weight): dq and dk came out 1.5 to 1.8 times (fp32: 6 times) as far from the exact ones
-// as plain arithmetic in 32 bits.  The kernels for few rows carry what the rounding of dS leaves off as a second operand,
-// and where no row can see more than 32 keys they form D by a walk of its own, one or two tiles long; small windows take them too.
+// Rows of few keys.  D = sum(dO O) does not cancel against dP as sum(P dP) does (two sums in different orders, which shows
+// where one key has nearly all the weight): dq and dk came out up to 6 times (fp32) as far from the exact ones as plain arithmetic
+// in 32 bits.  Where no row can see more than 32 keys the kernels for few rows form D by a walk of its own over them.
 bool fine(const WaP& p) { return std::min<int64_t>((int64_t)p.left + p.right + 1 + p.sinks, p.Tk) <= 32; }
 
 #define WA_DH(FN, T)                                                              \
@@ -1066,7 +1072,7 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     DTT_CHECK(g, "dtt_wattn_fwd: null argument");
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_fwd")) return rc;
-    DTT_CHECK(g->out && aligned16(g->out), "dtt_wattn_fwd: null or unaligned output");
+    DTT_CHECK(g->out && aligned16(g->out) && aligned16(p.rest), "dtt_wattn_fwd: null or unaligned output");
     const bool split = split_rows(p);
     const int bm = split ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
@@ -1095,8 +1101,8 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     DTT_CHECK(g, "dtt_wattn_bwd: null argument");
     WaP p;
     if (int rc = wa_check(g, p, "dtt_wattn_bwd")) return rc;
-    DTT_CHECK(g->out && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
-    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(g->dout) && aligned16(g->dq) &&
+    DTT_CHECK(g->out && (p.rest || g->dtype == 0) && g->dout && g->lse && g->dd && g->dq && g->dk && g->dv, "dtt_wattn_bwd: null buffer");
+    DTT_CHECK((p.g_sb | p.g_st | p.g_sh) % (g->dtype ? 8 : 4) == 0 && aligned16(g->out) && aligned16(p.rest) && aligned16(g->dout) && aligned16(g->dq) &&
               aligned16(g->dk) && aligned16(g->dv), "dtt_wattn_bwd: rows must start on 16 bytes");
     far_chunks(p);
     const int64_t need = part_bytes(p, g->DH);

@@ -116,7 +116,7 @@ class DttRotary(C.Structure):
 
 
 class DttWattn(C.Structure):
-    _fields_ = _fields("q k v out lse dout dq dk dv dd lengths ws".split(),
+    _fields_ = _fields("q k v out rest lse dout dq dk dv dd lengths ws".split(),
                        "ws_bytes q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh g_sb g_st g_sh".split(),
                        "B Tq Tk Hq Hk DH left right sinks offset dtype".split(), ("scale",))
 

@@ -271,28 +271,31 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
     g = DttWattn(B=B, Tq=Tq, Tk=k.shape[1], Hq=Hq, Hk=k.shape[2], DH=dh, left=cfg[0], right=cfg[1], sinks=cfg[2], offset=cfg[3],
                  dtype=1 if q.dtype is BF16 else 0, scale=cfg[4])
     _attn_inputs(g, q, k, v, lengths)
-    out, lse = torch.empty_like(q, memory_format=_ROWS), None
+    out, rest, lse = torch.empty_like(q, memory_format=_ROWS), None, None
     g.out = out.data_ptr()
     if keep:
+        if q.dtype is BF16:                                 # what rounding leaves off `out`: the gradients take it whole
+            rest = torch.empty_like(out)
+            g.rest = rest.data_ptr()
         lse = torch.empty((1 if q.dtype is BF16 else 2, B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
     check(lib().dtt_wattn_fwd(_addr(g), _stream(q.get_device())), "dtt_wattn_fwd")
-    return out, lse, g
+    return out, rest, lse, g
 
 
 class WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, cfg):
-        out, lse, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
-        ctx.save_for_backward(q, k, v, lengths, out, lse)
+        out, rest, lse, ctx.call = _attn_forward(q, k, v, lengths, cfg, True)
+        ctx.save_for_backward(q, k, v, lengths, out, rest, lse)
         return out
 
     @_first_order
     def backward(ctx, do):
-        q, k, v, lengths, out, lse = ctx.saved_tensors
+        q, k, v, lengths, out, rest, lse = ctx.saved_tensors
         q, k, v, do, g = _rows_attn(q), _rows_attn(k), _rows_attn(v), _rows_attn(do), _again(ctx.call)
         _attn_inputs(g, q, k, v, lengths)
-        g.out, g.lse = out.data_ptr(), lse.data_ptr()
+        g.out, g.rest, g.lse = out.data_ptr(), None if rest is None else rest.data_ptr(), lse.data_ptr()
         dq, dk, dv = (torch.empty_like(t, memory_format=_ROWS) for t in (q, k, v))
         dd = torch.empty_like(lse[0])
         g.dout, g.dq, g.dk, g.dv, g.dd = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dd.data_ptr()

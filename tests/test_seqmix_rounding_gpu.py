@@ -24,7 +24,8 @@ def rounded_once(got, ref, err, what):
 
 
 def bounds(q, k, v, see, scale, do):
-    """o, dv [B, T, H, dh] in float64 with the errors their kernels may have ahead of the final rounding."""
+    """o, dq, dk, dv [B, T, H, dh] in float64 with the errors their kernels may have ahead of the final rounding.  D is the sum of
+    dO O with O in two pieces, or of P dP: what moves O or a weight moves either by as much, its products' sums add (dh + 4) U."""
     B, Tq, Hq, dh = q.shape
     n, Hk = k.shape[1:3]
     G = Hq // Hk
@@ -39,12 +40,20 @@ def bounds(q, k, v, see, scale, do):
     back = lambda t, H, T: t.reshape(B, H, T, dh).transpose(1, 2)  # noqa: E731
     o, eo = P @ vd, (w + PIECES + n * U) * (P @ vd.abs())
     dv, edv = (P.transpose(-1, -2) @ dd).sum(2), ((P * (w + PIECES + Tq * G * U)).transpose(-1, -2) @ dd.abs()).sum(2)
-    return {"o": (back(o, Hq, Tq), back(eo, Hq, Tq)), "dv": (back(dv, Hk, n), back(edv, Hk, n))}
+    dP, mP = dd @ vd.transpose(-1, -2), dd.abs() @ vd.abs().transpose(-1, -2)
+    D = (dd * o).sum(-1, keepdim=True)
+    eD = (dd.abs() * (eo + PIECES * o.abs())).sum(-1, keepdim=True) + 2 * (dh + 4) * U * (P * mP).sum(-1, keepdim=True)
+    dS, mS = P * (dP - D), P * (dP - D).abs()
+    eS = P * ((dh + 4) * U * mP + eD) + (w + 8 * U + PIECES) * mS
+    dq, edq = dS @ kd * scale, (eS + n * U * mS) @ kd.abs() * scale
+    dk, edk = (dS.transpose(-1, -2) @ qd).sum(2) * scale, ((eS + Tq * G * U * mS).transpose(-1, -2) @ qd.abs()).sum(2) * scale
+    return {"o": (back(o, Hq, Tq), back(eo, Hq, Tq)), "dq": (back(dq, Hq, Tq), back(edq, Hq, Tq)),
+            "dk": (back(dk, Hk, n), back(edk, Hk, n)), "dv": (back(dv, Hk, n), back(edv, Hk, n))}
 
 
-def case(B, T, Hq, Hk, dh):
-    """Scores of half a standard deviation: their own errors stay far below a weight's rounding to bfloat16."""
-    q, k = (rnd(s, B, T, h, dh, dt=BF, std=0.5, grad=True) for s, h in ((1, Hq), (2, Hk)))
+def case(B, T, Hq, Hk, dh, std=0.5):
+    """Scores below a standard deviation: their own errors stay far below a weight's rounding to bfloat16."""
+    q, k = (rnd(s, B, T, h, dh, dt=BF, std=std, grad=True) for s, h in ((1, Hq), (2, Hk)))
     return q, k, rnd(3, B, T, Hk, dh, dt=BF, grad=True), rnd(4, B, T, Hq, dh, dt=BF)
 
 
@@ -62,6 +71,16 @@ def test_attention_and_values_gradient_are_rounded_once(dh, B, T, Hq, Hk, left, 
     want = bounds(q, k, v, seen(T, T, left, right, sinks, 0, None, B), dh ** -0.5, do)
     rounded_once(o, *want["o"], "o")
     rounded_once(dv, *want["dv"], "dv")
+
+
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,T,Hq,Hk,left,right,sinks", CASES)
+def test_attention_score_gradients_are_rounded_once(dh, B, T, Hq, Hk, left, right, sinks):
+    q, k, v, do = case(B, T, Hq, Hk, dh, 0.25)
+    dq, dk = torch.autograd.grad(A().window_attention(q, k, v, left, right, sinks), (q, k), do)
+    want = bounds(q, k, v, seen(T, T, left, right, sinks, 0, None, B), dh ** -0.5, do)
+    rounded_once(dq, *want["dq"], "dq")
+    rounded_once(dk, *want["dk"], "dk")
 
 
 @pytest.mark.parametrize("dh", [32, 64, 96, 128])
