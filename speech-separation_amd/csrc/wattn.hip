@@ -33,7 +33,7 @@ struct WaP {
     const int* len;
     int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, g_sb, g_st, g_sh;
     int B, Tq, Tk, Hq, Hk, G, left, right, sinks, offset;
-    int nt, few, nchunk, chunk, npart, edge;          // tiles along the row axis; chunks of the rows from edge on (first tokens' gradients)
+    int nt, nchunk, chunk, npart, edge;          // tiles along the row axis; chunks of the rows from edge on (first tokens' gradients)
     float scale;
 };
 
@@ -379,9 +379,14 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     }
 }
 
-// dq, and D = sum(dO O) per row for the dk / dv launch behind it
+// dq, and D per row for the dk / dv launch behind it.  D = sum(dO O) = sum(P dP).  The first, by the matrix cores as the diagonal of
+// O dO^T, costs nothing; bf16 takes O with what its rounding left off, since D cancels against dP, which is not rounded to 8 bits.
+// In fp32 it does not cancel as the second does (two sums in different orders, which shows where one key has nearly all the weight: dq
+// and dk of rows of two or three keys came out 2 to 6 times as far from the exact ones as plain arithmetic in 32 bits), so
+// workgroups in which a row sees no more than WALK_KEYS keys walk their keys, a few tiles, once more ahead for D = sum(P dP).
+constexpr int WALK_KEYS = 32;
 template <typename T, int DH, int RG, int SP>
-__global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_dq_kernel(const WaP p) {
+__global__ __launch_bounds__(NTH, SP == 1 && (sizeof(T) == 2 || DH <= 64) ? 2 : 1) void wattn_dq_kernel(const WaP p) {
     typedef Img<T, DH> I;
     typedef typename MM<T>::Frag Frag;
     constexpr int BM = 32 * RG, BN = SP == 1 ? 32 : 64;
@@ -407,9 +412,8 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
         gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
     }
-    // D = sum(dO O) by the matrix cores, as the diagonal of O dO^T (bf16: of O and what its rounding left off: D cancels against
-    // dP, which is not rounded to 8 bits); or, where rows see few keys, by a walk of its own over the keys as sum(P dP), see fine()
-    const bool walk = SP == 2 && p.few;
+    bool walk = false;
+    if constexpr (sizeof(T) == 4) walk = __syncthreads_or(live && seen_keys(p, pos, klen) <= WALK_KEYS);
     float dd = 0.f;
     if (!walk) {
         f32x16_t t = zero_acc();
@@ -439,38 +443,56 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 && SP == 1 ? 2 : 1) void wattn_
         sk.load(kp, p.k_st, r0, klen);
         sv.load(v, p.v_st, r0, klen);
     };
-    if (count > 0) load(0);
-    for (int w = walk ? -count : 0; w < count; ++w) {                       // w < 0: the walk for D
-        const int n = w < 0 ? w + count : w;
-        if (walk && w == 0) {                                               // both waves' halves of D
-            dd = both_sum(dd);
-            half[wave][lr] = dd;
-            __syncthreads();
-            dd = half[rg][lr] + half[(rg + RG) % (NTH / 64)][lr];
-        }
+    // tile n into LDS, the next one on its way; returns its first key
+    auto stage = [&](int n, int next) {
         __syncthreads();
         sk.store(ks);
         sv.store(vs);
         __syncthreads();
-        const int j0 = (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
-        if (w + 1 < count) load(n + 1 < count ? n + 1 : 0);
+        if (next < count) load(next);
+        return (n < tl.a ? n : tl.b + (n - tl.a)) * BN;
+    };
+    // any of the 32 keys from js on is visible
+    auto seen = [&](int js) { return !(js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen); };
+    // adds raw scores (hidden ones -inf) and dP of the staged 32 keys from 32 s on, key js the first
+    auto scores = [&](int s, int js, f32x16_t& x, f32x16_t& y) {
 #pragma unroll
-        for (int k = 0; k < BN / 32 / SP; ++k) {
-            const int s = k * SP + sp, js = j0 + 32 * s;
-            if (js > pw + 31 + p.right || (js + 31 < pw - p.left && js >= p.sinks) || js >= klen) continue;
-            f32x16_t x = zero_acc(), y = zero_acc();
+        for (int c = 0; c < DH / 16; ++c) {
+            MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
+            MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
+        }
+        const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
+        if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
+    };
+    if (count > 0) load(0);
+    if (walk) {
+        for (int n = 0; n < count; ++n) {
+            const int j0 = stage(n, n + 1 < count ? n + 1 : 0);             // (and the first tile again for the loop below)
 #pragma unroll
-            for (int c = 0; c < DH / 16; ++c) {
-                MM<T>::mma(nat_frag<T, DH>(ks, 32 * s + lr, c, lh), qf[c], x);
-                MM<T>::mma(nat_frag<T, DH>(vs, 32 * s + lr, c, lh), gf[c], y);
-            }
-            const bool full = js + 31 <= pw + p.right && (js >= pw + 31 - p.left || js + 31 < p.sinks) && js + 31 < klen;
-            if (!full) hide_keys(p, x, js + 4 * lh, pos, klen);
-            if (w < 0) {
+            for (int k = 0; k < BN / 32 / SP; ++k) {
+                const int s = k * SP + sp;
+                if (!seen(j0 + 32 * s)) continue;
+                f32x16_t x = zero_acc(), y = zero_acc();
+                scores(s, j0 + 32 * s, x, y);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dd = fmaf(__builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse) - lsum), y[r], dd);
-                continue;
             }
+        }
+        dd = both_sum(dd);
+        if constexpr (SP > 1) {                                             // both waves' halves
+            half[wave][lr] = dd;
+            __syncthreads();
+            dd = half[rg][lr] + half[(rg + RG) % (NTH / 64)][lr];
+        }
+    }
+    for (int n = 0; n < count; ++n) {
+        const int j0 = stage(n, n + 1);
+#pragma unroll
+        for (int k = 0; k < BN / 32 / SP; ++k) {
+            const int s = k * SP + sp;
+            if (!seen(j0 + 32 * s)) continue;
+            f32x16_t x = zero_acc(), y = zero_acc();
+            scores(s, j0 + 32 * s, x, y);
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], sc, -lse) - lsum) * (y[r] - dd);
             const Frag pf[2] = {acc_frag<T>(x, 0), acc_frag<T>(x, 1)};
@@ -1053,10 +1075,9 @@ int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk
 // the other way: forward 69 -> 85 us at 2 x 4096 rows, 16 / 4 heads.  512 workgroups are two a CU.
 bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
 bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
-// Rows of few keys.  D = sum(dO O) does not cancel against dP as sum(P dP) does (two sums in different orders, which shows
-// where one key has nearly all the weight): dq and dk came out up to 6 times (fp32) as far from the exact ones as plain arithmetic
-// in 32 bits.  Where no row can see more than 32 keys the kernels for few rows form D by a walk of its own over them.
-bool fine(const WaP& p) { return std::min<int64_t>((int64_t)p.left + p.right + 1 + p.sinks, p.Tk) <= 32; }
+// Windows of at most 32 keys: of the rows that a tile of 128 keys walks a wave's 32 keys are seen by few; tiles of 64: dk / dv
+// 92 -> 68 us at 8 x 4096 rows, 8 heads of 64, 8 keys, bf16 (fp32, half as many: 131 -> 125).
+bool narrow(const WaP& p) { return std::min<int64_t>((int64_t)p.left + p.right + 1 + p.sinks, p.Tk) <= 32; }
 
 #define WA_DH(FN, T)                                                              \
     do {                                                                          \
@@ -1109,8 +1130,7 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     DTT_CHECK(need == 0 || (g->ws && aligned16(g->ws) && g->ws_bytes >= need), "dtt_wattn_bwd: workspace of %lld bytes, %lld given",
               (long long)need, (long long)g->ws_bytes);
     p.part = (float*)g->ws;
-    p.few = fine(p);
-    const bool split = split_rows(p) || p.few, splitk = split_keys(p) || p.few;
+    const bool split = split_rows(p), splitk = split_keys(p) || narrow(p);
     const int bm = split ? 64 : 128, km = splitk ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
     WaP pk = p;
