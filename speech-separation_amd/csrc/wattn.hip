@@ -628,19 +628,20 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             if (far && (it || wave >= QN / 32)) continue;
             const int pr = p.offset + i0 + 32 * s;                        // position of the tile's first row
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
-            int vr = vrow;
-            // (the addresses of K's and V's fragments are formed anew for every tile: kept in registers they were spilled)
-            if constexpr (KL) asm volatile("" : "+v"(vr));
+            int vr = vrow, qr = 32 * s + lr;
+            // (the addresses of these fragments are formed anew for every tile: kept in registers they were spilled)
+            if constexpr (KL || (VL && sizeof(T) == 4)) asm volatile("" : "+v"(vr));
+            if constexpr (VL && sizeof(T) == 4) asm volatile("" : "+v"(qr));
             f32x16_t x = zero_acc(), y = zero_acc();
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
-                if constexpr (KL) MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), nat_frag<T, DH>(kimg, vr, c, lh), x);
-                else MM<T>::mma(nat_frag<T, DH>(qs, 32 * s + lr, c, lh), kf[c], x);
+                if constexpr (KL) MM<T>::mma(nat_frag<T, DH>(qs, qr, c, lh), nat_frag<T, DH>(kimg, vr, c, lh), x);
+                else MM<T>::mma(nat_frag<T, DH>(qs, qr, c, lh), kf[c], x);
             }
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
-                if constexpr (VL) MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), nat_frag<T, DH>(vimg, vr, c, lh), y);
-                else MM<T>::mma(nat_frag<T, DH>(gs, 32 * s + lr, c, lh), vf[c], y);
+                if constexpr (VL) MM<T>::mma(nat_frag<T, DH>(gs, qr, c, lh), nat_frag<T, DH>(vimg, vr, c, lh), y);
+                else MM<T>::mma(nat_frag<T, DH>(gs, qr, c, lh), vf[c], y);
             }
             const bool full = kw + 31 <= pr + p.right && (kw >= pr + 31 - p.left || kw + 31 < p.sinks) && kw + 31 < klen;
             if (!full) {                          // rows p with j - right <= p <= j + left (a first token: no end), one comparison
