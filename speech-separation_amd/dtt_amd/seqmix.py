@@ -25,6 +25,9 @@ from ._lib import lib, check, dtype_code, DttError, DttRecurrence, DttRotary, Dt
 
 F32, BF16, F64, I32, I64 = torch.float32, torch.bfloat16, torch.float64, torch.int32, torch.int64
 _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+# tells autograd that tensors were overwritten (through their addresses, which it cannot see): a backward pass that saved one of
+# them, or a view of it, then raises as it does behind any in-place operation
+_overwritten = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 _ROWS = torch.contiguous_format
 _addr = C.addressof
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):
@@ -252,6 +255,7 @@ def gated_recurrence_step(x, f, state):
                                        1 if dt is BF16 else 0, _stream(dev))
         if rc:
             check(rc, "dtt_recurrence_step")
+        _overwritten((state,))
     return y
 
 
@@ -418,6 +422,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, sinks=0, scale=N
     lib_, ref = lib(), _addr(g)
     ws = _workspace(g, lib_.dtt_wattn_step_ws_bytes(ref), q.device)  # noqa: F841 (alive until the call returns)
     check(lib_.dtt_wattn_step(ref, _stream(dev)), "dtt_wattn_step")
+    _overwritten((k_cache, v_cache))
     return out
 
 
@@ -442,6 +447,7 @@ def window_cache_fill(k, v, k_cache, v_cache, sinks=0, lengths=None):
     g.v_sb, g.v_st, g.v_sh, _ = v.stride()
     check(lib().dtt_wattn_cache_fill(_addr(g), None if lengths is None else lengths.data_ptr(), k.shape[1],
                                      _stream(k.get_device())), "dtt_wattn_cache_fill")
+    _overwritten((k_cache, v_cache))
 
 
 # --------------------------------------------------------------------------- #

@@ -1,0 +1,38 @@
+"""How the token mixers' calls that replace tensors in place, and arguments that could want a gradient, meet autograd."""
+import pytest
+import torch
+from test_seqmix_gpu import A, BF, DEV, F32, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_state_that_was_stepped_on_is_not_read_by_a_backward_pass():
+    """The recurrence saves its h0 for the backward pass; a step replaces the same tensor: an error, as behind state.copy_()."""
+    x, f = rnd(1, 2, 9, 8, grad=True), rnd(2, 2, 9, 8, grad=True)
+    state = rnd(3, 2, 8)
+    y, _ = A().gated_recurrence(x, f, state)
+    with torch.no_grad():
+        A().gated_recurrence_step(x[:, 0], f[:, 0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y, _ = A().gated_recurrence(x, f, state.clone())                          # of a copy: as ever
+    want = torch.autograd.grad(y.sum(), f, retain_graph=True)[0]
+    with torch.no_grad():
+        A().gated_recurrence_step(x[:, 0], f[:, 0], state)
+    assert torch.equal(torch.autograd.grad(y.sum(), f)[0], want)
+
+
+@pytest.mark.parametrize("how", ["step", "fill"])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_caches_that_were_written_are_not_read_by_a_backward_pass(dt, how):
+    q, kc, vc = rnd(1, 2, 5, 2, 32, dt=dt, grad=True), rnd(2, 2, 20, 2, 32, dt=dt), rnd(3, 2, 20, 2, 32, dt=dt)
+    k, v = rnd(4, 2, 2, 32, dt=dt), rnd(5, 2, 2, 32, dt=dt)
+    for keys, values in ((kc[:, 3:17], vc.clone()[:, 3:17]), (kc.clone()[:, 3:17], vc[:, 3:17])):      # views of either cache
+        o = A().window_attention(q, keys, values, 4)
+        with torch.no_grad():
+            if how == "step":
+                A().window_attention_step(q[:, 0], k, v, kc, vc, torch.tensor([4, 5], device=DEV))
+            else:
+                A().window_cache_fill(k[:, None], v[:, None], kc, vc)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.sum().backward()
