@@ -378,6 +378,8 @@ def _step_args(name, k, v, k_cache, v_cache, sinks, scale):
         _fail(name, "caches must have the dtype of k")
     if k_cache.get_device() != k.get_device() or v_cache.get_device() != k.get_device():
         _fail(name, "caches must be on the device of k")
+    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad):
+        _fail(name, "no gradient through caches: call it under torch.no_grad()")
     if not 0 <= sinks < cs[1] or cs[1] >> 30:
         _fail(name, f"sinks={sinks} of {cs[1]} slots (at least one for the window, less than 2^30)")
     g = DttWattnStep(B=cs[0], Hq=cs[2], Hk=cs[2], DH=cs[3], S=sinks, W=cs[1] - sinks, dtype=1 if k.dtype is BF16 else 0, scale=scale)

@@ -36,3 +36,15 @@ def test_caches_that_were_written_are_not_read_by_a_backward_pass(dt, how):
                 A().window_cache_fill(k[:, None], v[:, None], kc, vc)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             o.sum().backward()
+
+
+def test_caches_in_a_graph_are_refused():
+    """Their gradient would miss what is written: refused while gradients are recorded, taken under no_grad."""
+    q, k = rnd(1, 1, 2, 32), rnd(2, 1, 2, 32)
+    kc, vc, pos = rnd(3, 1, 6, 2, 32, grad=True), rnd(4, 1, 6, 2, 32), torch.zeros(1, dtype=torch.int64, device=DEV)
+    for a, b in ((kc, vc), (vc, kc), (kc * 1, vc)):
+        for call in (lambda: A().window_attention_step(q, k, k, a, b, pos), lambda: A().window_cache_fill(k[:, None], k[:, None], a, b)):
+            with pytest.raises(A().DttError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
