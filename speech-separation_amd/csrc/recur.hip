@@ -453,8 +453,10 @@ __global__ __launch_bounds__(NTH) void rec_bwd_kernel(const RecP p) {
             for (int v = 0; v < VEC; ++v) {
                 const float gt = g[i][v] + sn[v];
                 sn[v] = a[i][v] * gt;
-                vx[v] = im[i][v] * gt;                                // (0 behind the length: im = 0)
-                vf[v] = im[i][v] * d[i][v] * sn[v];
+                // (behind the length 0 whatever dlast and the state are: im = 0 times one that is not finite is not)
+                const bool live = full || t + i < w.len;
+                vx[v] = live ? im[i][v] * gt : 0.f;
+                vf[v] = live ? im[i][v] * d[i][v] * sn[v] : 0.f;
             }
             ox[i].put(vx);
             of[i].put(vf);

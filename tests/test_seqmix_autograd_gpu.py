@@ -48,3 +48,28 @@ def test_caches_in_a_graph_are_refused():
                 call()
             with torch.no_grad():
                 call()
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("N,L,D", [(4, 20, 6), (4, 4000, 16), (1040, 12, 256)])
+def test_padding_has_no_gradient_when_the_state_is_not_finite(N, L, D, dt, reverse):
+    """One time lane, tiles of eight lanes, segments: gradients behind an item's length are 0 whatever passes there, and items and
+    channels whose state is finite get the gradients that they get alone."""
+    x, f = rnd(1, N, L, D, dt=dt, grad=True), rnd(2, N, L, D, dt=dt, mean=2.0, grad=True)
+    h0, dy, dl = rnd(3, N, D), rnd(4, N, L, D, dt=dt), rnd(5, N, D)
+    lens = torch.randint(0, L + 1, (N,), generator=torch.Generator().manual_seed(1))
+    lens[:4] = torch.tensor([0, L, L // 2, 1])
+    lens = lens.to(DEV)
+    clean = torch.autograd.grad(A().gated_recurrence(x, f, h0, reverse, lens), (x, f), (dy, dl))
+    bad, badl = h0.clone(), dl.clone()
+    bad[0, 0], bad[2, 1], bad[3, 2] = float("inf"), float("nan"), float("-inf")
+    badl[0, 3], badl[2, 4], badl[3, 5] = float("nan"), float("inf"), float("nan")
+    dirty = torch.zeros(N, D, dtype=torch.bool, device=DEV)
+    dirty[[0, 0, 2, 2, 3, 3], [0, 3, 1, 4, 2, 5]] = True
+    got = torch.autograd.grad(A().gated_recurrence(x, f, bad, reverse, lens), (x, f), (dy, badl))
+    pad = (torch.arange(L, device=DEV)[None] >= lens[:, None])[..., None].expand(N, L, D)
+    for g, c in zip(got, clean):
+        assert not g[pad].any()
+        fine = ~dirty[:, None].expand(N, L, D)
+        assert torch.equal(g[fine], c[fine])
