@@ -520,7 +520,7 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
 
     q [B, T, Hq, dh] and k [B, T, Hk, dh] (or None) of one dtype; positions int64 or int32 [T] or [B, T]; freq float64
     (rotary_frequencies).  Angles are formed in float64, so positions far into a stream keep their precision.  Returns the
-    turned q and k (or q alone where k is None); differentiable in both."""
+    turned q and k (or q alone where k is None); differentiable in both, not in freq."""
     name = "rotary"
     if not torch.is_tensor(q) or q.dim() != 4:
         _fail(name, "q must be [B, T, H, dh]")
@@ -537,6 +537,8 @@ def rotary(q, k, positions, freq, interleaved=False, amplitude=1.0):
         _fail(name, f"positions must be int32 or int64 [T] or [B, T], got {positions.dtype} {tuple(positions.shape)}")
     if freq.dtype is not F64 or freq.dim() != 1 or not freq.is_contiguous() or not 0 < 2 * freq.shape[0] <= min(dh, 4096):
         _fail(name, "freq must be a contiguous float64 vector of 1 to dh / 2 elements (2048 at most)")
+    if freq.requires_grad and torch.is_grad_enabled():
+        _fail(name, "no gradient of freq: detach it")
     if positions.get_device() != dev or freq.get_device() != dev:
         _fail(name, f"positions and freq must be on {q.device}")
     if q.numel() == 0 or (k is not None and k.numel() == 0):

@@ -73,3 +73,14 @@ def test_padding_has_no_gradient_when_the_state_is_not_finite(N, L, D, dt, rever
         assert not g[pad].any()
         fine = ~dirty[:, None].expand(N, L, D)
         assert torch.equal(g[fine], c[fine])
+
+
+def test_frequencies_that_want_a_gradient_are_refused():
+    freq, pos = A().rotary_frequencies(32, device=DEV).requires_grad_(), torch.arange(4, device=DEV)
+    q = rnd(1, 1, 4, 2, 32)
+    for t in (q, rnd(1, 1, 4, 2, 32, grad=True)):
+        with pytest.raises(A().DttError, match="gradient of freq"):
+            A().rotary(t, t, pos, freq)
+    with torch.no_grad():
+        a = A().rotary(q, q, pos, freq)
+    assert all(torch.equal(x, y) for x, y in zip(a, A().rotary(q, q, pos, freq.detach())))
