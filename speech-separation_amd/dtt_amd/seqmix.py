@@ -364,7 +364,8 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, offset=None,
     if dev != _device():
         with torch.cuda.device(dev):
             return window_attention(q, k, v, left, right, sinks, lengths, offset, scale)
-    cfg = (min(left, _BIG), min(right, _BIG), sinks, offset, q.shape[-1] ** -0.5 if scale is None else float(scale))
+    # (positions reach offset + Tq < 2^29: a window cut to less than that would hide keys)
+    cfg = (min(left, 2 * _BIG - 1), min(right, _BIG), sinks, offset, q.shape[-1] ** -0.5 if scale is None else float(scale))
     q, k, v = _rows_attn(q), _rows_attn(k), _rows_attn(v)
     return WindowAttention.apply(q, k, v, lengths, cfg) if grad else _attn_forward(q, k, v, lengths, cfg, False)[0]
 
