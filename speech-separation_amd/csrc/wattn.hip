@@ -1176,12 +1176,23 @@ int ws_check(const DttWattnStep* g, WsP& p, const char* what) {
               (g->dtype ? 8 : 4) == 0 && aligned16(g->q) && aligned16(g->k) && aligned16(g->v) && aligned16(g->kc) && aligned16(g->vc),
               "%s: rows must start on 16 bytes", what);
     p.B = g->B; p.Hq = g->Hq; p.Hk = g->Hk; p.G = g->Hq / g->Hk; p.ngrp = (p.G + 31) / 32; p.S = g->S; p.W = g->W; p.scale = g->scale;
-    // splits of the slots: where there is less than a workgroup a CU, ranges of 512 slots at least (four tiles a wave).  One a
-    // CU reads at the full rate already: 64 streams over 4016 slots, 16 / 4 heads of 128, 93 us, with four splits 99 + 6
+    // Splits of the slots, in ranges of 512 at least (four tiles a wave).  One workgroup a CU reads at the full rate: 64 streams over
+    // 4016 slots, 16 / 4 heads of 128, 93 us, with four splits 99 + 6.  Up to half as many (item, key head) pairs as CUs are split
+    // until that is reached.  Above, the busiest CU decides: it has ceil(rows n / 256) of n parts, and two or three are
+    // taken where that is less by a fifth, the join and the shorter ranges costing as much (same heads, us: 132 pairs 78 whole, 85 in two,
+    // 63 in three; 160: 80, 89, 70; 192: 83, 93, 91; 264: 158, 132, 116; 384: 175, 154; 416: 180, 184; 512: 204, 203).  The fp32
+    // kernel, twice the waves a workgroup, gains from parts of less than 1024 slots only above 256 pairs (2016 slots, heads of 64: 132
+    // pairs 42 whole, 45 in three; 264: 90, 75).
     const int M = g->S + g->W;
-    const int64_t rows = (int64_t)p.B * p.Hk * p.ngrp;
-    int64_t ns = 256 / rows, most = (M + 511) / 512;
-    ns = ns < 1 ? 1 : ns > most ? most : ns;
+    const int64_t rows = (int64_t)p.B * p.Hk * p.ngrp, most = (M + 511) / 512;
+    int64_t ns = std::min(256 / rows, most);
+    if (ns < 2) {
+        const auto busiest = [&](int64_t n) { return (rows * n + 255) / 256 * (6 / n); };        // in sixths of a row
+        const int64_t least = g->dtype || rows > 256 ? 512 : 1024;
+        ns = 1;
+        for (int64_t n = 2; n <= 3 && n <= (M + least - 1) / least; ++n)
+            if (busiest(n) * 5 <= busiest(1) * 4 && busiest(n) < busiest(ns)) ns = n;
+    }
     p.per = (int)(((M + ns - 1) / ns + 127) / 128 * 128);
     p.nsplit = (M + p.per - 1) / p.per;
     return 0;
