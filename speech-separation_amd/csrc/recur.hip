@@ -453,13 +453,17 @@ __global__ __launch_bounds__(NTH) void rec_bwd_kernel(const RecP p) {
             for (int v = 0; v < VEC; ++v) {
                 const float gt = g[i][v] + sn[v];
                 sn[v] = a[i][v] * gt;
-                // (behind the length 0 whatever dlast and the state are: im = 0 times one that is not finite is not)
-                const bool live = full || t + i < w.len;
-                vx[v] = live ? im[i][v] * gt : 0.f;
-                vf[v] = live ? im[i][v] * d[i][v] * sn[v] : 0.f;
+                vx[v] = im[i][v] * gt;
+                vf[v] = im[i][v] * d[i][v] * sn[v];
             }
             ox[i].put(vx);
             of[i].put(vf);
+        }
+        if (!full) {                                                  // behind the length 0, also where im = 0 met a state or dlast that is not finite
+            const float zero[VEC] = {};
+#pragma unroll
+            for (int i = 0; i < TC; ++i)
+                if (t + i >= w.len) ox[i].put(zero), of[i].put(zero);
         }
         w.store(p, dx, t, te, full, ox);
         w.store(p, df, t, te, full, of);
