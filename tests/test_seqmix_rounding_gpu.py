@@ -121,3 +121,24 @@ def test_float32_rows_of_few_keys_in_a_wide_window(B, T, H, dh):
     for g, p, e, name in zip(got, plain, exact, ("dq", "dk")):
         mine, theirs = float((g.cpu().double() - e)[:, :4].norm()), float((p - e)[:, :4].norm())
         assert mine <= 1.5 * theirs, (name, mine, theirs, mine / theirs)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("start", [0, 20_000_000])
+def test_float32_rotary_with_whole_angles(inter, start):
+    """In 2-norm over half a million elements no further off than plain float32 with sines and cosines rounded from float64: the
+    kernel's own may be an ulp off, a rounding more beside the three of the products and their sum: sqrt(4 / 3), 1.16.  (A
+    fraction of a turn rounded to float32 first: 1.3.)"""
+    q = rnd(1, 2, 2003, 2, 64)
+    freq, pos = A().rotary_frequencies(64, device=DEV), start + torch.arange(2003, device=DEV)
+    got = A().rotary(q, None, pos, freq, interleaved=inter)
+    ang = (pos.double()[:, None] * freq)[:, None]
+    c, s = torch.cos(ang), torch.sin(ang)
+
+    def turned(x, c, s):
+        u, v = (x[..., 0::2], x[..., 1::2]) if inter else (x[..., :32], x[..., 32:])
+        pair = u * c - v * s, u * s + v * c
+        return torch.stack(pair, -1).flatten(-2) if inter else torch.cat(pair, -1)
+
+    exact, plain = turned(q.double(), c, s), turned(q, c.float(), s.float())
+    assert float((got - exact).norm()) <= 1.16 * float((plain - exact).norm())
