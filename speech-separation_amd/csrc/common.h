@@ -179,5 +179,7 @@ inline void dtt_want_lds(const void* fn, int bytes) {
     }
 }
 
+// a launch has fewer than 2^32 threads
+#define DTT_MAX_THREADS (1ll << 32)
 #define DTT_LAUNCH_CHECK() do { hipError_t e__ = hipGetLastError(); if (e__ != hipSuccess) { \
     dtt_set_error("%s:%d launch failed: %s", __FILE__, __LINE__, hipGetErrorString(e__)); return -2; } } while (0)

@@ -543,7 +543,7 @@ int fill(RecP& p, const DttRecurrence* g, Plan& q, const char* what) {
     DTT_CHECK(g->L <= (1 << 30), "%s: L=%d, at most 2^30", what, g->L);
     DTT_CHECK(g->dtype == 0 || g->dtype == 1, "%s: dtype must be 0 (float32) or 1 (bfloat16)", what);
     DTT_CHECK(g->x && g->f, "%s: null buffer", what);
-    DTT_CHECK(q.groups < (1ll << 31), "%s: too many columns", what);
+    DTT_CHECK(q.groups * NTH < DTT_MAX_THREADS, "%s: too many columns", what);
     const int64_t need = q.nseg > 1 ? (int64_t)q.nseg * 2 * g->N * g->D * 4 : 0;
     DTT_CHECK(need == 0 || (g->ws && g->ws_bytes >= need), "%s: workspace of %lld bytes, %lld given", what, (long long)need,
               (long long)g->ws_bytes);
@@ -623,7 +623,7 @@ extern "C" int dtt_recurrence_step(const void* x, const void* f, float* state, v
                       (uintptr_t)state % 16 == 0;
     const int dv = wide ? D / 4 : D;
     const int64_t cols = (int64_t)N * dv;
-    DTT_CHECK(cols < (1ll << 38), "dtt_recurrence_step: too many columns");
+    DTT_CHECK(cols + NTH < DTT_MAX_THREADS, "dtt_recurrence_step: too many columns");
     const dim3 grid((unsigned)((cols + NTH - 1) / NTH));
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define STEP(T, V) hipLaunchKernelGGL((rec_step_kernel<T, V>), grid, dim3(NTH), 0, s, (const T*)x, (const T*)f, state, (T*)y, cols, dv, x_sn, f_sn, D)

@@ -111,13 +111,14 @@ extern "C" int dtt_rotary(const DttRotary* g, void* stream) {
     int vec = 16 / e;
     while (vec > 1 && (str % vec || ad % (vec * e))) vec /= 2;
     // tokens of a workgroup: about four passes of the threads over its items, no more than leaves four workgroups a CU
-    const int64_t items = (int64_t)(g->Hq + g->Hk) * ((g->interleaved ? g->r : g->r / 2) + g->dh - g->r) / vec;
+    const int64_t items = ((int64_t)g->Hq + g->Hk) * ((g->interleaved ? g->r : g->r / 2) + g->dh - g->r) / vec;
     int64_t tok = (4 * NTH + items - 1) / items;
     if (tok > p.n / 1024) tok = p.n / 1024;
     if (tok > 4096 / p.r) tok = 4096 / p.r;
     p.tok = tok < 1 ? 1 : (int)tok;
     const int64_t grid = (p.n + p.tok - 1) / p.tok;
-    DTT_CHECK(grid < (1ll << 31), "dtt_rotary: too many tokens");
+    DTT_CHECK(grid * NTH < DTT_MAX_THREADS, "dtt_rotary: too many tokens");
+    DTT_CHECK(items * p.tok < (1ll << 31) - NTH, "dtt_rotary: too many heads");        // (a workgroup counts its items in 32 bits)
     const size_t lds = (size_t)p.tok * (p.r / 2) * sizeof(float2);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define ROT(T, V, I) hipLaunchKernelGGL((rotary_kernel<T, V, I>), dim3((unsigned)grid), dim3(NTH), lds, s, p)

@@ -1099,7 +1099,7 @@ extern "C" int dtt_wattn_fwd(const DttWattn* g, void* stream) {
     const int bm = split ? 64 : 128;
     p.nt = (p.Tq + bm - 1) / bm;
     const int64_t grid = (int64_t)p.B * p.Hq * p.nt;
-    DTT_CHECK(grid < (1ll << 31), "dtt_wattn_fwd: too many rows");
+    DTT_CHECK(grid * NTH < DTT_MAX_THREADS, "dtt_wattn_fwd: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define FWD(T, D)                                                                                                      \
     do {                                                                                                               \
@@ -1138,7 +1138,8 @@ extern "C" int dtt_wattn_bwd(const DttWattn* g, void* stream) {
     pk.nt = (p.Tk + km - 1) / km;
     const int64_t gq = (int64_t)p.B * p.Hq * p.nt, gk = (int64_t)p.B * p.Hk * pk.nt;
     const int64_t gf = (int64_t)p.B * p.Hk * p.nchunk * ((p.sinks + 31) / 32), n = (int64_t)p.B * p.Hk * p.sinks * 2 * g->DH;
-    DTT_CHECK(gq < (1ll << 31) && gk + gf < (1ll << 31), "dtt_wattn_bwd: too many rows");
+    DTT_CHECK(gq * NTH < DTT_MAX_THREADS && (gk + gf) * (splitk || g->dtype == 0 ? NTH : 2 * NTH) < DTT_MAX_THREADS && (n + 63) / 64 * NTH < DTT_MAX_THREADS,
+              "dtt_wattn_bwd: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const dim3 dq((unsigned)gq), dkv((unsigned)(gk + gf));
 #define BWD(T, D)                                                                                                                  \
@@ -1216,7 +1217,8 @@ extern "C" int dtt_wattn_step(const DttWattnStep* g, void* stream) {
               (long long)g->ws_bytes);
     p.part = (float*)g->ws;
     const int64_t grid = (int64_t)p.B * p.Hk * p.ngrp * p.nsplit, n = (int64_t)p.B * p.Hq * g->DH;
-    DTT_CHECK(grid < (1ll << 31) && n < (1ll << 38), "dtt_wattn_step: too many rows");
+    DTT_CHECK(grid * (g->dtype == 0 && p.G <= 4 ? 512 : NTH) < DTT_MAX_THREADS && (p.nsplit == 1 || n + NTH < DTT_MAX_THREADS),
+              "dtt_wattn_step: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define STEP(T, D) hipLaunchKernelGGL((wattn_step_kernel<T, D>), dim3((unsigned)grid), dim3(NTH), 0, s, p)
 #define FEW1(D, N) hipLaunchKernelGGL((wattn_step_few_kernel<D, N>), dim3((unsigned)grid), dim3(512), 0, s, p)
@@ -1247,7 +1249,7 @@ extern "C" int dtt_wattn_cache_fill(const DttWattnStep* g, const int32_t* length
     DTT_CHECK(Tn == 1 || (g->k_st | g->v_st) % (g->dtype ? 8 : 4) == 0, "dtt_wattn_cache_fill: rows must start on 16 bytes");
     const int np = g->DH / (g->dtype ? 8 : 4);
     const int64_t n = (int64_t)p.B * (p.S + p.W) * p.Hk * np, grid = (n + NTH - 1) / NTH;
-    DTT_CHECK(grid < (1ll << 31), "dtt_wattn_cache_fill: too many rows");
+    DTT_CHECK(grid * NTH < DTT_MAX_THREADS, "dtt_wattn_cache_fill: too many rows");
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (g->dtype) hipLaunchKernelGGL((wattn_fill_kernel<bf16>), dim3((unsigned)grid), dim3(NTH), 0, s, p, lengths, Tn, g->k_st, g->v_st, np, n);
     else hipLaunchKernelGGL((wattn_fill_kernel<float>), dim3((unsigned)grid), dim3(NTH), 0, s, p, lengths, Tn, g->k_st, g->v_st, np, n);

@@ -22,3 +22,29 @@ def test_splits_of_a_frame(pairs, splits, dtype):
             assert got == splits
         if slots == 1024 and dtype == 0 and 128 < pairs <= 256:
             assert got == 1
+
+
+def test_sizes_beyond_a_launch():
+    """2^32 threads and more, or a rotary workgroup of 2^31 items, are refused by name."""
+    from dtt_amd._lib import DttRecurrence, DttRotary, DttWattn, DttWattnStep, lib
+    L = lib()
+
+    def refused(rc, part):
+        assert rc == -1 and part in L.dtt_last_error().decode(), (rc, L.dtt_last_error())
+
+    a = DttWattn(q=BUF, k=BUF, v=BUF, out=BUF, rest=BUF, lse=BUF, dout=BUF, dq=BUF, dk=BUF, dv=BUF, dd=BUF, B=1 << 20, Tq=1, Tk=1, Hq=16, Hk=16, DH=32,
+                 left=3, scale=1.0, dtype=1, q_sb=512, q_sh=32, k_sb=512, k_sh=32, v_sb=512, v_sh=32, g_sb=512, g_sh=32)
+    refused(L.dtt_wattn_fwd(C.byref(a), None), "too many rows")
+    refused(L.dtt_wattn_bwd(C.byref(a), None), "too many rows")
+    s = DttWattnStep(q=BUF, k=BUF, v=BUF, kc=BUF, vc=BUF, out=BUF, positions=BUF, B=1 << 20, Hq=16, Hk=16, DH=32, S=0, W=1, scale=1.0, dtype=1,
+                     q_sb=512, q_sh=32, k_sb=512, k_sh=32, v_sb=512, v_sh=32, kc_sb=512, kc_st=512, kc_sh=32, vc_sb=512, vc_st=512, vc_sh=32)
+    refused(L.dtt_wattn_step(C.byref(s), None), "too many rows")
+    s.B, s.W = 1, 1 << 26
+    refused(L.dtt_wattn_cache_fill(C.byref(s), None, 5, None), "too many rows")
+    r = DttRecurrence(x=BUF, f=BUF, y=BUF, x_so=1 << 16, f_so=1 << 16, N=1 << 17, NI=1, L=1, D=1 << 16)
+    refused(L.dtt_recurrence_fwd(C.byref(r), None), "too many columns")
+    refused(L.dtt_recurrence_step(BUF, BUF, BUF, BUF, 1 << 18, 1 << 16, 1 << 16, 1 << 16, 1, None), "too many columns")
+    t = DttRotary(q=BUF, qo=BUF, positions=BUF, freq=BUF, B=1, T=1, Hq=1 << 26, dh=66, r=2, q_sh=66, amplitude=1.0, dtype=1)
+    refused(L.dtt_rotary(C.byref(t), None), "too many heads")
+    t = DttRotary(q=BUF, qo=BUF, positions=BUF, freq=BUF, B=1 << 16, T=1 << 16, Hq=1 << 12, dh=32, r=32, q_sb=32, q_st=32, q_sh=32, amplitude=1.0)
+    refused(L.dtt_rotary(C.byref(t), None), "too many tokens")
