@@ -13,10 +13,11 @@
 // whatever the window (o 2.22e-3 against 1.63e-3 relative, dv 2.33e-3 and dq 2.42e-3 against 1.66e-3).  Statistics,
 // accumulators, D = sum(dO O) and first tokens' partial sums stay fp32.
 //
-// Bound: the matrix cores (4 DH flops per visible pair forward, 10 DH backward) for windows beyond a few hundred keys, HBM
-// below.  Measured, bf16, 2 x 4096 rows, 16 / 4 heads of 128, window 512 + 4 first tokens (114 GF, 92 us at the rate of a
-// large matrix product): forward 66 us, dq 86, dk / dv 129, the first tokens' sums 5.  What keeps them from it are
-// latencies in series (staging, Q K^T, exponentials, P V) at the two waves a SIMD that the accumulators leave room for.
+// Bound: the matrix cores (4 DH flops per visible pair forward, 10 DH backward; in bf16 the second operands add 2 and 6 that the
+// formulas do not have) for windows beyond a few hundred keys, HBM below.  Measured, bf16, 2 x 4096 rows, 16 / 4 heads of 128,
+// window 512 + 4 first tokens (114 GF, 92 us at the rate of a large matrix product): forward 77 us (85 with what the backward pass
+// wants of it), dq 103, dk / dv 156, the first tokens' sums 5; matrix cores busy 26 to 30 % of the time.  What keeps them from the
+// rate are latencies in series (staging, Q K^T, exponentials, the pieces, P V) at the two waves a SIMD that the accumulators leave room for.
 #include "common.h"
 #include "../../include/dtt_hip.h"
 #include <algorithm>
@@ -1072,12 +1073,12 @@ void far_chunks(WaP& p) {
 int64_t part_bytes(const WaP& p, int dh) { return p.nchunk ? (int64_t)p.B * p.Hk * p.npart * p.sinks * 2 * dh * 4 : 0; }
 
 // Few rows: half of them a workgroup, two waves on each (the walk over its keys half as long): fp32 training over 16 clips of
-// 376 frames, 2 heads of 128: forward 45 -> 24 us, dq 60 -> 34, dk / dv 85 -> 37; with 1024 workgroups, two to four a CU,
-// the other way: forward 69 -> 85 us at 2 x 4096 rows, 16 / 4 heads.  512 workgroups are two a CU.
+// 376 frames, 2 heads of 128: forward 44 -> 23 us, dq 67 -> 37, dk / dv 77 -> 38; with 1024 workgroups, two to four a CU,
+// the other way: 2 x 4096 rows, 16 / 4 heads, bf16: forward 85 -> 98 us, dq 104 -> 198, dk / dv 157 -> 204.  512 workgroups are two a CU.
 bool split_rows(const WaP& p) { return (int64_t)p.B * p.Hq * ((p.Tq + 127) / 128) < 512; }
 bool split_keys(const WaP& p) { return (int64_t)p.B * p.Hk * ((p.Tk + 127) / 128) < 256; }
 // Windows of at most 32 keys: of the rows that a tile of 128 keys walks a wave's 32 keys are seen by few; tiles of 64: dk / dv
-// 92 -> 68 us at 8 x 4096 rows, 8 heads of 64, 8 keys, bf16 (fp32, half as many: 131 -> 125).
+// 91 -> 68 us at 8 x 4096 rows, 8 heads of 64, 8 keys, bf16 (fp32, half as many: 132 -> 126).
 bool narrow(const WaP& p) { return std::min<int64_t>((int64_t)p.left + p.right + 1 + p.sinks, p.Tk) <= 32; }
 
 #define WA_DH(FN, T)                                                              \
