@@ -492,7 +492,7 @@ int dtt_rotary(const DttRotary* g, void* stream);
  * take no part in the gradients.  q, dout [B][Tq][Hq][DH], k, v [B][Tk][Hk][DH] by strides (rows of one head DH to 2^22
  * elements apart, every row on 16 bytes); out, dq [B][Tq][Hq][DH] and dk, dv [B][Tk][Hk][DH] contiguous; Hq a multiple of
  * Hk; DH 32, 64, 96 or 128; sinks <= 128; scale > 0.
- * lse [B][Hq][Tq], in float32 [2][B][Hq][Tq] (forward: may be NULL): base-2 log of each row's sum, for the backward call;
+ * lse [2][B][Hq][Tq] (forward: may be NULL): each row's softmax reference and the base-2 log of its sum, for the backward call;
  * rest [B][Tq][Hq][DH] (bfloat16 only; forward: may be NULL): what the rounding of out left off, for the backward call;
  * dd [B][Hq][Tq]: scratch of the backward call; ws: dtt_wattn_bwd_ws_bytes() bytes, scratch.  No atomics: equal calls give
  * equal bits. */

@@ -373,18 +373,17 @@ __global__ __launch_bounds__(NTH, sizeof(T) == 2 ? 2 : 1) void wattn_fwd_kernel(
     }
     store_rows<T, DH>((T*)p.out + row, o, live ? 1.f / l : 0.f, lh, p.rest ? (T*)p.rest + row : nullptr);
     if (p.lse && lh == 0) {
-        // (fp32: reference and log of the sum apart, their sum as one float would cost the weights 2^-24 of its size)
+        // (reference and log of the sum apart: their sum as one float would cost the weights 2^-24 of its size)
         float* s = p.lse + ((int64_t)b * p.Hq + h) * p.Tq + i;
-        if constexpr (sizeof(T) == 4) s[0] = live ? m : INFINITY, s[(int64_t)p.B * p.Hq * p.Tq] = live ? log2f(l) : 0.f;
-        else s[0] = live ? m + log2f(l) : INFINITY;
+        s[0] = live ? m : INFINITY, s[(int64_t)p.B * p.Hq * p.Tq] = live ? log2f(l) : 0.f;
     }
 }
 
 // dq, and D per row for the dk / dv launch behind it.  D = sum(dO O) = sum(P dP).  The first, by the matrix cores as the diagonal of
 // O dO^T, costs nothing; bf16 takes O with what its rounding left off, since D cancels against dP, which is not rounded to 8 bits.
-// In fp32 it does not cancel as the second does (two sums in different orders, which shows where one key has nearly all the weight: dq
-// and dk of rows of two or three keys came out 2 to 6 times as far from the exact ones as plain arithmetic in 32 bits), so
-// workgroups in which a row sees no more than WALK_KEYS keys walk their keys, a few tiles, once more ahead for D = sum(P dP).
+// It does not cancel as the second does (two sums in different orders, and O's own errors, which show where one key has nearly all
+// the weight: fp32 dq of rows of two or three keys came out 2 to 6 times as far from the exact one as plain arithmetic in 32 bits),
+// so workgroups in which a row sees no more than WALK_KEYS keys walk their keys, a few tiles, once more ahead for D = sum(P dP).
 constexpr int WALK_KEYS = 32;
 template <typename T, int DH, int RG, int SP>
 __global__ __launch_bounds__(NTH, SP == 1 && (sizeof(T) == 2 || DH <= 64) ? 2 : 1) void wattn_dq_kernel(const WaP p) {
@@ -413,8 +412,7 @@ __global__ __launch_bounds__(NTH, SP == 1 && (sizeof(T) == 2 || DH <= 64) ? 2 : 
         qf[c] = MM<T>::ldfrag(q + 16 * c + 8 * lh);
         gf[c] = MM<T>::ldfrag(go + 16 * c + 8 * lh);
     }
-    bool walk = false;
-    if constexpr (sizeof(T) == 4) walk = __syncthreads_or(live && seen_keys(p, pos, klen) <= WALK_KEYS);
+    const bool walk = __syncthreads_or(live && seen_keys(p, pos, klen) <= WALK_KEYS);
     float dd = 0.f;
     if (!walk) {
         f32x16_t t = zero_acc();
@@ -428,7 +426,7 @@ __global__ __launch_bounds__(NTH, SP == 1 && (sizeof(T) == 2 || DH <= 64) ? 2 : 
         dd = both_sum(dd);
     }
     const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + ic;
-    const float lse = p.lse[at], lsum = sizeof(T) == 4 ? p.lse[at + (int64_t)p.B * p.Hq * p.Tq] : 0.f;
+    const float lse = p.lse[at], lsum = p.lse[at + (int64_t)p.B * p.Hq * p.Tq];
     f32x16_t dq[DH / 32];
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) dq[c] = zero_acc();
@@ -542,7 +540,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
     constexpr int PARK = SP > 1 ? KG * DH * 128 / (int)sizeof(T) : 0;
     static_assert(SP <= QN / 32, "a 32-row tile of a staged one for every wave that shares keys");
     __shared__ __align__(16) T mem[N > PARK ? N : PARK];
-    __shared__ __align__(16) float st[sizeof(T) == 4 ? 4 : 3][QN];        // per row: log of the sum, D, and 1 (0 where one key is seen: no gradient of weights)
+    __shared__ __align__(16) float st[sizeof(T) == 4 ? 4 : 3][QN];        // per row: reference, D, 1 (0 where one key is seen: no gradient of weights), log of the sum
     T* qs = mem;
     T* gs = mem + TILE;
     T* vimg = mem + 2 * TILE;
@@ -605,7 +603,7 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             const int i = r + threadIdx.x;
             const int64_t at = ((int64_t)b * p.Hq + h) * p.Tq + min(i, p.Tq - 1);
             const float lv = p.lse[at], dvv = p.dd[at];
-            if constexpr (sizeof(T) == 4) ss = p.lse[at + (int64_t)p.B * p.Hq * p.Tq];
+            ss = p.lse[at + (int64_t)p.B * p.Hq * p.Tq];
             sl = i < r1 ? lv : INFINITY;
             sw = i < r1 && seen_keys(p, p.offset + i, klen) > 1 ? 1.f : 0.f;
             sd = sw != 0.f ? dvv : 0.f;
@@ -617,7 +615,8 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
         sq.store(qs);
         sg.store(gs);
         if (threadIdx.x < QN) {
-            st[0][threadIdx.x] = sl, st[1][threadIdx.x] = sd, st[2][threadIdx.x] = sw;
+            // (bf16: the two as one float; D is formed already, and a weight's own 2^-24 of that is far below its pieces)
+            st[0][threadIdx.x] = sizeof(T) == 4 ? sl : sl + ss, st[1][threadIdx.x] = sd, st[2][threadIdx.x] = sw;
             if constexpr (sizeof(T) == 4) st[3][threadIdx.x] = ss;
         }
         __syncthreads();
@@ -631,8 +630,8 @@ __global__ __launch_bounds__(KG * SP * 64, sizeof(T) == 2 && (DH <= 64 || KG * S
             if (kw > pr + 31 + p.right || (kw + 31 < pr - p.left && kw >= p.sinks) || kw >= klen || i0 + 32 * s >= r1) continue;
             int vr = vrow, qr = 32 * s + lr;
             // (the addresses of these fragments are formed anew for every tile: kept in registers they were spilled)
-            if constexpr (KL || (VL && sizeof(T) == 4)) asm volatile("" : "+v"(vr));
-            if constexpr (VL && sizeof(T) == 4) asm volatile("" : "+v"(qr));
+            if constexpr (VL) asm volatile("" : "+v"(vr));
+            if constexpr (VL && !KL) asm volatile("" : "+v"(qr));
             f32x16_t x = zero_acc(), y = zero_acc();
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {

@@ -281,7 +281,7 @@ def _attn_forward(q, k, v, lengths, cfg, keep):
         if q.dtype is BF16:                                 # what rounding leaves off `out`: the gradients take it whole
             rest = torch.empty_like(out)
             g.rest = rest.data_ptr()
-        lse = torch.empty((1 if q.dtype is BF16 else 2, B, Hq, Tq), dtype=F32, device=q.device)
+        lse = torch.empty((2, B, Hq, Tq), dtype=F32, device=q.device)
         g.lse = lse.data_ptr()
     check(lib().dtt_wattn_fwd(_addr(g), _stream(q.get_device())), "dtt_wattn_fwd")
     return out, rest, lse, g

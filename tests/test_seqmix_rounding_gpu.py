@@ -142,3 +142,30 @@ def test_float32_rotary_with_whole_angles(inter, start):
 
     exact, plain = turned(q.double(), c, s), turned(q, c.float(), s.float())
     assert float((got - exact).norm()) <= 1.16 * float((plain - exact).norm())
+
+
+@pytest.mark.parametrize("B,T,H,dh", [(16, 100, 8, 64), (64, 140, 4, 128)])
+@pytest.mark.parametrize("left,rows", [(1, 100), (7, 100), (200, 20)])
+@pytest.mark.parametrize("spread", [3.0, 8.0])
+def test_rows_with_nearly_all_weight_on_one_key(B, T, H, dh, left, rows, spread):
+    """Their gradients are small differences: dP - D, where D has to be the sum of P dP with the very weights that dS is formed
+    from, and those have to sum to 1 as closely as float32 lets them.  Errors row by row, relative to the row, rounded to bfloat16 at
+    the end: 99 of 100 rows no worse than 1.5 times what plain float32 gives for 99 of 100 (the same float32 roundings, at most
+    twice as many).  Of the rows whose gradient float32 resolves: it is 1 - P of the one key's dP - D, which carries a few U of dP in any
+    float32 arithmetic, so a row counts where 1 - P is at least 2^-12.  (Below 2^-24 plain float32 rounds P to 1 and the gradient
+    to 0, off by exactly 1 of it, and any rounding elsewhere, however small, by more.)"""
+    q, k, v = (rnd(s, B, T, H, dh, dt=BF, std=std, grad=True) for s, std in ((1, spread), (2, 1.0), (3, 1.0)))
+    do = rnd(4, B, T, H, dh, dt=BF)
+    got, = torch.autograd.grad(A().window_attention(q, k, v, left), q, do)
+    see = seen(T, T, left, 0, 0, 0, None, 1)
+    exact, plain = (plain_score_gradients(q, k, v, do, see, dh ** -0.5, dt)[0][:, 1:rows] for dt in (F64, torch.float32))
+    s = torch.einsum("bthd,bshd->bths", q.detach().double(), k.detach().double()) * dh ** -0.5
+    top = torch.softmax(torch.where(see[:, :, None], s, -math.inf), -1).topk(2, -1).values
+    counts = (top[..., 1] >= 2.0 ** -12)[:, 1:rows].cpu()
+    assert int(counts.sum()) > 1000
+
+    def worst(t):
+        e = (t.to(BF).double() - exact).norm(dim=-1) / exact.norm(dim=-1)
+        return float(torch.quantile(e[counts], 0.99))
+
+    assert worst(got.cpu()[:, 1:rows]) <= 1.5 * worst(plain), (worst(got.cpu()[:, 1:rows]), worst(plain))
